@@ -202,7 +202,7 @@ def prepare(case, seed):
         s["cap"] = max(1, int(counts.max()))
     s["slot"] = slot.to(DEV)
     c, b = _codes(_randn(g, rows, K), fmt, af)
-    s["a"] = _pack(c).reshape(*shape, K // 2)
+    s["a"] = _pack(c).byte().reshape(*shape, K // 2)
     s["sfa"] = torch.stack([_tile(x, fmt) for x in b.reshape(G, M, -1)]) if case["layout"] == "masked" else _tile(b, fmt)
     s["d"] = torch.zeros((*shape, N), dtype=DT[case["out"]], device=DEV)
     return s
