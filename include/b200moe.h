@@ -31,6 +31,7 @@ extern "C" {
 
 #define MOE_DTYPE_BF16 0
 #define MOE_DTYPE_F32 1
+#define MOE_DTYPE_F16 2
 
 #define MOE_SF_F32 0            /* block scales as fp32 values */
 #define MOE_SF_UE8M0_PACKED 1   /* block scales as UE8M0 bytes, four consecutive 128-K blocks per int32 */
@@ -227,6 +228,152 @@ int moe_permute(const void* x_q, const float* x_scale, int64_t xs_row, int64_t x
  * (output.index_add_(0, token_idx, O * w_tok) ... .to(bfloat16)). */
 int moe_combine(const void* y_bf16, const int32_t* pos, const float* w, void* out_bf16, int32_t T, int32_t top_k,
                 int32_t H, void* stream);
+
+/* ---- what stands before the layer: norm, routing; 4-bit operands ----------------------------- */
+
+/* Residual addition, root-mean-square norm and 1x128 quantisation in one pass over the row:
+ *   h = round(x + residual) in x's type;  rstd = (mean(h^2) + eps)^(-1/2);  y = h * rstd * weight
+ *   per 128 columns (the last block may be shorter): s = max(amax|y|, 1e-8) / 448 and q = e4m3(y / s), as
+ *   moe_quant_1x128 does; pow2 != 0: s is rounded up to a power of two, the scales that let the grouped GEMM apply them
+ *   inside the tensor core.
+ * x, residual [T, H] of `dtype` (bf16, f16 or f32), unit column stride, row strides in elements (multiples of 8);
+ * weight [H] of w_dtype (dtype or f32).  residual may be NULL (then h is x, and h is not written).  h and y (may be NULL:
+ * the unquantised output) are dense [T, H] of `dtype`; q dense e4m3 [T, H]; scales at [r * ss_row + block * ss_blk];
+ * rstd f32 [T].  H % 8 == 0, H <= 16384; pointers 16-byte aligned.  Sums are kept in fp32.  h and y may not overlap the inputs.
+ * A row with a NaN or an infinity has NaN in its scales and codes.  The reference has no counterpart. */
+typedef struct moe_norm_args {
+    const void* x;
+    int64_t x_stride;
+    const void* residual;
+    int64_t residual_stride;
+    const void* weight;
+    void* q;
+    float* scales;
+    int64_t ss_row, ss_blk;
+    void* h;
+    void* y;
+    float* rstd;
+    int32_t T, H, dtype, w_dtype, pow2;
+    float eps;
+} moe_norm_args;
+int moe_rms_norm_quant(const moe_norm_args* args, void* stream);
+
+/* Gradient of the norm above, the rounding to 8 bits passed through unchanged: with dy = dL/dy,
+ *   dx = rstd * (dy w - n mean(dy w n)) (+ dh),  n = h * rstd      -- the gradient of x and of residual alike
+ *   dw = sum over rows of dy * n                                   -- f32, always added up in the same order
+ * dy, h [T, H] of dtype and dh (may be NULL; the gradient that reaches h past the norm) with row strides as above; dx
+ * dense [T, H] of dtype; dw f32 [H]; rstd f32 [T] from the forward call.  workspace: 16-byte aligned. */
+typedef struct moe_norm_grad_args {
+    const void* dy;
+    int64_t dy_stride;
+    const void* h;
+    int64_t h_stride;
+    const void* weight;
+    const float* rstd;
+    const void* dh;
+    int64_t dh_stride;
+    void* dx;
+    float* dw;
+    int32_t T, H, dtype, w_dtype;
+    void* workspace;
+    uint64_t workspace_bytes;
+} moe_norm_grad_args;
+size_t moe_rms_norm_backward_workspace_bytes(int32_t T, int32_t H);
+int moe_rms_norm_backward(const moe_norm_grad_args* args, void* stream);
+
+/* Top-k routing: score p = softmax(logits) or sigmoid(logits); the experts are chosen by p + bias (bias may be NULL) and
+ * weighted by p alone.  n_group > 1: only experts of the topk_group best groups (E / n_group consecutive experts each)
+ * can be chosen; a group counts for its best p + bias or, with MOE_GROUP_TOP2, the sum of its two best.
+ * weights = p * scale, or with renormalize p / (sum of the chosen p + 1e-20) * scale.
+ * logits [T, E] of `dtype` (bf16, f16, f32), row stride in elements; bias [E] bf16 or f32; ids int32 and weights f32
+ * [T, top_k], in descending order of p + bias.  The order is the exact one of p + bias, ties to the lowest index.
+ * A logit of -infinity or NaN (and a bias that is not finite) switches its expert off; where fewer than top_k are left
+ * the id is -1 and the weight 0, and moe_permute_plan drops the pair.  E <= 1024, top_k <= min(32, E), n_group <= 32.
+ * The general form of moe_route_topk and moe_route_deepseek (fp32 logits; their fixed rules). */
+#define MOE_SCORE_SOFTMAX 0
+#define MOE_SCORE_SIGMOID 1
+#define MOE_GROUP_MAX 0
+#define MOE_GROUP_TOP2 1
+typedef struct moe_route_args {
+    const void* logits;
+    int64_t stride;
+    const void* bias;
+    int32_t* ids;
+    float* weights;
+    int32_t T, E, top_k, n_group, topk_group, dtype, bias_dtype, score, group_score, renormalize;
+    float scale;
+} moe_route_args;
+int moe_route(const moe_route_args* args, void* stream);
+
+/* Gradient of the weights with respect to the logits, ids held fixed: dlogits dense [T, E] of dtype.  An id outside
+ * [0, E) or of an expert that is switched off is skipped; an id that a token holds twice counts twice. */
+typedef struct moe_route_grad_args {
+    const float* grad_weights;    /* [T, top_k] */
+    const void* logits;
+    int64_t stride;
+    const int32_t* ids;           /* [T, top_k] */
+    void* dlogits;
+    int32_t T, E, top_k, dtype, score, renormalize;
+    float scale;
+} moe_route_grad_args;
+int moe_route_backward(const moe_route_grad_args* args, void* stream);
+
+/* 4-bit block formats.  Codes are e2m1 (0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives), two to a byte, the earlier
+ * in the low half.
+ *   MOE_FP4_NV  one e4m3 scale s per 16 values and one fp32 factor g: value = code * s * g; quantisation takes
+ *               s = e4m3(min(amax / (6 g), 448)), code = e2m1(x / (s g))
+ *   MOE_FP4_MX  one UE8M0 scale per 32 values: s = 2^(floor(log2 amax) - 2), at least 2^-127; code = e2m1(x / s)
+ * (round to nearest even; magnitudes above 6 become 6).  A block that holds an infinity or a NaN gets the scale NaN.
+ * Scales lie in tiles of 512 bytes for 128 rows x 4 blocks: uint8 [row blocks of 128][ceil(K/256) * (4 NV, 2 MX)][512],
+ * row r's four bytes at (r % 32) * 16 + (r / 32) * 4.  A matrix of several groups ([G, rows, K]) has row blocks of its
+ * own for each group. */
+#define MOE_FP4_NV 0
+#define MOE_FP4_MX 1
+
+/* x [groups * src_rows, K] ([.., 2K] with silu_mul: act = SiLU(gate) * up in fp32 is quantised; gate_first as in
+ * moe_silu_mul_requant) of `dtype`, row stride in elements (multiple of 8) -> codes q [groups, rows, K/2] and scales.
+ *   src_pair  may be NULL (then rows == src_rows).  int32 [rows], groups == 1: row r is made from row src_pair[r] / top_k
+ *             of x, as moe_permute gathers; negative: neither the row's codes nor its scales are written
+ *   factor    g of group i at factor[i * factor_stride], positive and finite; NULL = 1 (MOE_FP4_MX: NULL)
+ * Scales of rows and blocks behind the last one are written as zero.  K % 128 == 0, pointers 16-byte aligned. */
+typedef struct moe_fp4_quant_args {
+    const void* x;
+    int64_t x_stride;
+    const float* factor;
+    int32_t factor_stride;
+    const int32_t* src_pair;
+    void* q;
+    void* scales;
+    int32_t groups, rows, src_rows, K, top_k, dtype, format, silu_mul, gate_first;
+} moe_fp4_quant_args;
+int moe_quant_fp4(const moe_fp4_quant_args* args, void* stream);
+
+/* The codes' values as e4m3 (which holds each of them): n_bytes of packed codes -> 2 * n_bytes of e4m3.  n_bytes % 8 == 0;
+ * pointers 16-byte aligned. */
+int moe_unpack_fp4(const void* q, void* out_e4m3, int64_t n_bytes, void* stream);
+
+/* m-grouped GEMM of 4-bit operands: D_g = alpha_g * deq(A_g) * deq(B_g)^T with fp32 accumulation.
+ *   a      codes [M, K/2] (contiguous) / [G, M, K/2] (masked, M = max rows per group), sfa its scale tiles
+ *   b      codes [G, N, K/2], sfb its scale tiles [G][ceil(N/128)]..
+ *   alpha  alpha[g * alpha_stride] (MOE_FP4_NV: the product of the two factors); NULL = 1
+ *   layout, d, ldd, d_dtype, rows_used as in moe_gg_args
+ * Rows of d that no group owns are left as they are.  K % 128 == 0, N % 8 == 0, ldd % 8 == 0, G <= 1024 (masked);
+ * a, b, sfa, sfb and d 16-byte aligned. */
+typedef struct moe_gg_fp4_args {
+    const void* a;
+    const void* sfa;
+    const void* b;
+    const void* sfb;
+    const float* alpha;
+    int32_t alpha_stride;
+    const int32_t* layout;
+    const int32_t* rows_used;
+    void* d;
+    int64_t ldd;
+    int32_t G, M, N, K, format, d_dtype;
+} moe_gg_fp4_args;
+int moe_gg_fp4_contiguous(const moe_gg_fp4_args* args, void* stream);
+int moe_gg_fp4_masked(const moe_gg_fp4_args* args, void* stream);
 
 /* ---- one MoE layer on one GPU --------------------------------------------------------------- */
 

@@ -75,6 +75,67 @@ class AlphaView(_c.Structure):
     _fields_ = [(n, _c.c_void_p) for n in ("counts", "rowpos", "s1", "s2", "g1", "d2", "a1", "a2")] + [("max_m", _c.c_int64)]
 
 
+class NormArgs(_c.Structure):
+    """``moe_norm_args`` of include/b200moe.h."""
+    _fields_ = [
+        ("x", _c.c_void_p), ("x_stride", _c.c_int64), ("residual", _c.c_void_p), ("residual_stride", _c.c_int64),
+        ("weight", _c.c_void_p), ("q", _c.c_void_p), ("scales", _c.c_void_p), ("ss_row", _c.c_int64), ("ss_blk", _c.c_int64),
+        ("h", _c.c_void_p), ("y", _c.c_void_p), ("rstd", _c.c_void_p),
+        ("T", _c.c_int32), ("H", _c.c_int32), ("dtype", _c.c_int32), ("w_dtype", _c.c_int32), ("pow2", _c.c_int32),
+        ("eps", _c.c_float),
+    ]
+
+
+class NormGradArgs(_c.Structure):
+    """``moe_norm_grad_args`` of include/b200moe.h."""
+    _fields_ = [
+        ("dy", _c.c_void_p), ("dy_stride", _c.c_int64), ("h", _c.c_void_p), ("h_stride", _c.c_int64),
+        ("weight", _c.c_void_p), ("rstd", _c.c_void_p), ("dh", _c.c_void_p), ("dh_stride", _c.c_int64),
+        ("dx", _c.c_void_p), ("dw", _c.c_void_p),
+        ("T", _c.c_int32), ("H", _c.c_int32), ("dtype", _c.c_int32), ("w_dtype", _c.c_int32),
+        ("workspace", _c.c_void_p), ("workspace_bytes", _c.c_uint64),
+    ]
+
+
+class RouteArgs(_c.Structure):
+    """``moe_route_args`` of include/b200moe.h."""
+    _fields_ = [
+        ("logits", _c.c_void_p), ("stride", _c.c_int64), ("bias", _c.c_void_p), ("ids", _c.c_void_p), ("weights", _c.c_void_p),
+        ("T", _c.c_int32), ("E", _c.c_int32), ("top_k", _c.c_int32), ("n_group", _c.c_int32), ("topk_group", _c.c_int32),
+        ("dtype", _c.c_int32), ("bias_dtype", _c.c_int32), ("score", _c.c_int32), ("group_score", _c.c_int32),
+        ("renormalize", _c.c_int32), ("scale", _c.c_float),
+    ]
+
+
+class RouteGradArgs(_c.Structure):
+    """``moe_route_grad_args`` of include/b200moe.h."""
+    _fields_ = [
+        ("grad_weights", _c.c_void_p), ("logits", _c.c_void_p), ("stride", _c.c_int64), ("ids", _c.c_void_p),
+        ("dlogits", _c.c_void_p), ("T", _c.c_int32), ("E", _c.c_int32), ("top_k", _c.c_int32), ("dtype", _c.c_int32),
+        ("score", _c.c_int32), ("renormalize", _c.c_int32), ("scale", _c.c_float),
+    ]
+
+
+class Fp4QuantArgs(_c.Structure):
+    """``moe_fp4_quant_args`` of include/b200moe.h."""
+    _fields_ = [
+        ("x", _c.c_void_p), ("x_stride", _c.c_int64), ("factor", _c.c_void_p), ("factor_stride", _c.c_int32),
+        ("src_pair", _c.c_void_p), ("q", _c.c_void_p), ("scales", _c.c_void_p),
+        ("groups", _c.c_int32), ("rows", _c.c_int32), ("src_rows", _c.c_int32), ("K", _c.c_int32), ("top_k", _c.c_int32),
+        ("dtype", _c.c_int32), ("format", _c.c_int32), ("silu_mul", _c.c_int32), ("gate_first", _c.c_int32),
+    ]
+
+
+class GGFp4Args(_c.Structure):
+    """``moe_gg_fp4_args`` of include/b200moe.h."""
+    _fields_ = [
+        ("a", _c.c_void_p), ("sfa", _c.c_void_p), ("b", _c.c_void_p), ("sfb", _c.c_void_p), ("alpha", _c.c_void_p),
+        ("alpha_stride", _c.c_int32), ("layout", _c.c_void_p), ("rows_used", _c.c_void_p), ("d", _c.c_void_p),
+        ("ldd", _c.c_int64), ("G", _c.c_int32), ("M", _c.c_int32), ("N", _c.c_int32), ("K", _c.c_int32),
+        ("format", _c.c_int32), ("d_dtype", _c.c_int32),
+    ]
+
+
 class EpPeers(_c.Structure):
     """``moe_ep_peers`` of include/b200moe.h."""
     _fields_ = [("a", _c.c_void_p * 8), ("sa", _c.c_void_p * 8), ("y", _c.c_void_p * 8),
@@ -121,6 +182,8 @@ EXPORTS = (
     "moe_gg_fp8_contiguous", "moe_gg_fp8_masked", "moe_gg_fp8_gate_up_act", "moe_gg_workspace_bytes", "moe_quant_1x128", "moe_silu_mul_requant",
     "moe_route_topk", "moe_route_deepseek", "moe_permute_workspace_bytes", "moe_permute_plan", "moe_permute_plan_static", "moe_permute",
     "moe_combine",
+    "moe_rms_norm_quant", "moe_rms_norm_backward_workspace_bytes", "moe_rms_norm_backward", "moe_route", "moe_route_backward",
+    "moe_quant_fp4", "moe_unpack_fp4", "moe_gg_fp4_contiguous", "moe_gg_fp4_masked",
     "moe_workspace_bytes", "moe_layer_forward", "moe_layer_workspace_view", "moe_device_status",
     "moe_alpha_workspace_bytes", "moe_alpha_forward", "moe_alpha_workspace_view",
     "moe_kg_workspace_bytes", "moe_kg_fp8_contiguous",
@@ -130,7 +193,12 @@ EXPORTS = (
     "moe_last_error", "moe_version",
 )
 _SIZE_T_RETURN = ("moe_gg_workspace_bytes", "moe_permute_workspace_bytes", "moe_workspace_bytes", "moe_ep_workspace_bytes",
-                  "moe_alpha_workspace_bytes", "moe_kg_workspace_bytes")
+                  "moe_alpha_workspace_bytes", "moe_kg_workspace_bytes", "moe_rms_norm_backward_workspace_bytes")
+
+
+# dtypes and modes of include/b200moe.h
+DTYPE_BF16, DTYPE_F32, DTYPE_F16 = range(3)
+FP4_NV, FP4_MX = range(2)
 
 
 # moe_set_option keys and values (include/b200moe.h)

@@ -20,6 +20,10 @@
 #include "alpha_moe.cuh"
 #include "alpha_gemm.cuh"
 #include "alpha_gemv.cuh"
+#include "norm_ops.cuh"
+#include "route_ops.cuh"
+#include "fp4_ops.cuh"
+#include "gg_fp4.cuh"
 
 namespace {
 
@@ -1445,3 +1449,5 @@ const char* moe_last_error(void) { return g_err; }
 const char* moe_version(void) { return "b200moe 0.1 sm_100a"; }
 
 }  // extern "C"
+
+#include "layer_ops_host.cuh"

@@ -1,0 +1,282 @@
+// Host side of the norm, routing and 4-bit entry points: validation and launches.  Included by b200moe.cu, whose error
+// reporting and device table it uses.
+#pragma once
+
+namespace {
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+inline bool float_dtype(int d) { return d == MOE_DTYPE_BF16 || d == MOE_DTYPE_F32 || d == MOE_DTYPE_F16; }
+inline int dtype_bytes(int d) { return d == MOE_DTYPE_F32 ? 4 : 2; }
+
+// f(a value of the element type)
+template <typename F>
+void with_dtype(int dtype, F f) {
+    if (dtype == MOE_DTYPE_BF16) f(__nv_bfloat16{});
+    else if (dtype == MOE_DTYPE_F16) f(__half{});
+    else f(float{});
+}
+
+int check_norm(int32_t T, int32_t H, int32_t dtype, int32_t w_dtype) {
+    if (T < 0 || H <= 0 || H % 8 || H > NORM_MAX_H)
+        return fail(MOE_ERR_INVALID, "T=%d must be non-negative and H=%d a multiple of 8 in [8, %d]", T, H, NORM_MAX_H);
+    if (!float_dtype(dtype) || (w_dtype != dtype && w_dtype != MOE_DTYPE_F32))
+        return fail(MOE_ERR_INVALID, "dtype must be bf16, f16 or f32, and w_dtype the same or f32");
+    return MOE_OK;
+}
+int check_rows(const char* name, const void* p, int64_t stride, int32_t H) {
+    if (!p) return fail(MOE_ERR_INVALID, "%s must be non-NULL", name);
+    if (!aligned16(p) || stride < H || stride % 8)
+        return fail(MOE_ERR_INVALID, "%s must be 16-byte aligned with a row stride >= H that is a multiple of 8", name);
+    return MOE_OK;
+}
+
+// Threads and 8-column pieces per thread: one piece up to 512 threads, then two or four.
+struct NormShape { int threads, pieces; };
+NormShape norm_shape(int H) {
+    const int n8 = H / 8;
+    NormShape s;
+    s.pieces = n8 <= NORM_MAX_THREADS ? 1 : (n8 <= 2 * NORM_MAX_THREADS ? 2 : 4);
+    s.threads = ((n8 + s.pieces - 1) / s.pieces + 31) / 32 * 32;
+    return s;
+}
+
+template <typename T, typename W>
+void launch_norm(const NormParams& p, NormShape s, cudaStream_t st) {
+    if (s.pieces == 1) rms_norm_quant_kernel<T, W, 1><<<p.T, s.threads, 0, st>>>(p);
+    else if (s.pieces == 2) rms_norm_quant_kernel<T, W, 2><<<p.T, s.threads, 0, st>>>(p);
+    else rms_norm_quant_kernel<T, W, 4><<<p.T, s.threads, 0, st>>>(p);
+}
+template <typename T, typename W>
+void launch_norm_grad(const NormGradParams& p, int grid, NormShape s, cudaStream_t st) {
+    if (s.pieces == 1) rms_norm_grad_kernel<T, W, 1><<<grid, s.threads, 0, st>>>(p);
+    else if (s.pieces == 2) rms_norm_grad_kernel<T, W, 2><<<grid, s.threads, 0, st>>>(p);
+    else rms_norm_grad_kernel<T, W, 4><<<grid, s.threads, 0, st>>>(p);
+}
+
+int check_route(int32_t T, int32_t E, int32_t top_k, int32_t dtype, int32_t score, int64_t stride) {
+    if (T < 0 || E <= 0 || E > RT_MAX_E) return fail(MOE_ERR_INVALID, "T=%d must be non-negative and E=%d in [1, %d]", T, E, RT_MAX_E);
+    if (top_k <= 0 || top_k > 32 || top_k > E) return fail(MOE_ERR_INVALID, "top_k=%d must be in [1, min(32, E)]", top_k);
+    if (!float_dtype(dtype)) return fail(MOE_ERR_INVALID, "dtype must be bf16, f16 or f32");
+    if (score != MOE_SCORE_SOFTMAX && score != MOE_SCORE_SIGMOID) return fail(MOE_ERR_INVALID, "score must be MOE_SCORE_SOFTMAX or MOE_SCORE_SIGMOID");
+    if (stride < E) return fail(MOE_ERR_INVALID, "stride=%lld must be >= E", (long long)stride);
+    return MOE_OK;
+}
+// whole 16-byte pieces of a row can be read (and written, in a dense output) wherever a lane's experts begin
+bool route_vec(const void* p, int64_t stride, int32_t E, int32_t dtype) {
+    const int n = 16 / dtype_bytes(dtype);
+    return aligned16(p) && stride % n == 0 && E % n == 0;
+}
+
+template <typename T>
+void launch_route(const RouteParams& p, size_t smem, cudaStream_t st) {
+    const int grid = (p.T + RT_WARPS - 1) / RT_WARPS, block = RT_WARPS * 32;
+    if (p.E <= 128) route_kernel<T, 4><<<grid, block, smem, st>>>(p);
+    else if (p.E <= 256) route_kernel<T, 8><<<grid, block, smem, st>>>(p);
+    else if (p.E <= 512) route_kernel<T, 16><<<grid, block, smem, st>>>(p);
+    else route_kernel<T, 32><<<grid, block, smem, st>>>(p);
+}
+template <typename T>
+void launch_route_grad(const RouteGradParams& p, cudaStream_t st) {
+    const int grid = (p.T + RT_WARPS - 1) / RT_WARPS, block = RT_WARPS * 32;
+    if (p.E <= 128) route_grad_kernel<T, 4><<<grid, block, 0, st>>>(p);
+    else if (p.E <= 256) route_grad_kernel<T, 8><<<grid, block, 0, st>>>(p);
+    else if (p.E <= 512) route_grad_kernel<T, 16><<<grid, block, 0, st>>>(p);
+    else route_grad_kernel<T, 32><<<grid, block, 0, st>>>(p);
+}
+
+template <typename T>
+void launch_quant_fp4(const Fp4QuantParams& p, bool nv, bool silu, dim3 grid, cudaStream_t st) {
+    if (nv && silu) quant_fp4_kernel<T, true, true><<<grid, FP4_QUANT_THREADS, 0, st>>>(p);
+    else if (nv) quant_fp4_kernel<T, true, false><<<grid, FP4_QUANT_THREADS, 0, st>>>(p);
+    else if (silu) quant_fp4_kernel<T, false, true><<<grid, FP4_QUANT_THREADS, 0, st>>>(p);
+    else quant_fp4_kernel<T, false, false><<<grid, FP4_QUANT_THREADS, 0, st>>>(p);
+}
+
+int launch_gg_fp4(const moe_gg_fp4_args* a, bool masked, void* stream) {
+    if (!a) return fail(MOE_ERR_INVALID, "args is NULL");
+    if (a->G <= 0 || a->N <= 0 || a->K <= 0 || a->M < 0)
+        return fail(MOE_ERR_INVALID, "G, N, K must be positive and M non-negative (G=%d M=%d N=%d K=%d)", a->G, a->M, a->N, a->K);
+    if (a->K % 128 != 0) return fail(MOE_ERR_INVALID, "K=%d must be a multiple of 128", a->K);
+    if (a->N % 8 != 0) return fail(MOE_ERR_INVALID, "N=%d must be a multiple of 8", a->N);
+    if (a->format != MOE_FP4_NV && a->format != MOE_FP4_MX) return fail(MOE_ERR_INVALID, "format must be MOE_FP4_NV or MOE_FP4_MX");
+    if (a->d_dtype != MOE_DTYPE_BF16 && a->d_dtype != MOE_DTYPE_F32) return fail(MOE_ERR_INVALID, "d_dtype must be MOE_DTYPE_BF16 or MOE_DTYPE_F32");
+    if (a->ldd < a->N || a->ldd % 8 != 0) return fail(MOE_ERR_INVALID, "ldd=%lld must be >= N and a multiple of 8", (long long)a->ldd);
+    if (masked && a->G > gg::MAX_MASKED_GROUPS) return fail(MOE_ERR_INVALID, "masked layout supports at most %d groups", gg::MAX_MASKED_GROUPS);
+    const long long rows_total = masked ? (long long)a->G * a->M : (long long)a->M;
+    if (rows_total > 0x7FFFFFFFll || (long long)a->G * a->N > 0x7FFFFFFFll) return fail(MOE_ERR_INVALID, "row counts exceed 2^31-1");
+    if (a->alpha && a->alpha_stride != 0 && a->alpha_stride != 1) return fail(MOE_ERR_INVALID, "alpha_stride must be 0 or 1");
+    if (rows_total == 0) return MOE_OK;
+    if (!a->a || !a->sfa || !a->b || !a->sfb || !a->layout || !a->d) return fail(MOE_ERR_INVALID, "a, sfa, b, sfb, layout and d must all be non-NULL");
+    if (!aligned16(a->a) || !aligned16(a->sfa) || !aligned16(a->b) || !aligned16(a->sfb) || !aligned16(a->d))
+        return fail(MOE_ERR_INVALID, "a, sfa, b, sfb and d must be 16-byte aligned");
+    DeviceInfo* di = nullptr;
+    int rc = device_info(&di);
+    if (rc != MOE_OK) return rc;
+    GGFp4Params p = {};
+    p.a = static_cast<const uint8_t*>(a->a); p.b = static_cast<const uint8_t*>(a->b);
+    p.sfa = static_cast<const uint8_t*>(a->sfa); p.sfb = static_cast<const uint8_t*>(a->sfb);
+    p.alpha = a->alpha; p.alpha_stride = a->alpha_stride;
+    p.layout = a->layout; p.rows_used = masked ? nullptr : a->rows_used;
+    p.d = a->d; p.ldd = a->ldd; p.d_f32 = a->d_dtype == MOE_DTYPE_F32;
+    p.G = a->G; p.M = a->M; p.N = a->N; p.K = a->K; p.masked = masked;
+    p.kt = (a->K + 255) / 256 * (a->format == MOE_FP4_NV ? 4 : 2);
+    p.a_tiles = (a->M + 127) / 128; p.b_tiles = (a->N + 127) / 128;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    dim3 grid((a->M + 63) / 64, (a->N + 63) / 64, masked ? a->G : 1);
+    if (a->format == MOE_FP4_NV) gg_fp4_simple_kernel<true><<<grid, 256, 0, st>>>(p);
+    else gg_fp4_simple_kernel<false><<<grid, 256, 0, st>>>(p);
+    CUDA_TRY(cudaGetLastError());
+    return MOE_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int moe_rms_norm_quant(const moe_norm_args* a, void* stream) {
+    if (!a) return fail(MOE_ERR_INVALID, "args is NULL");
+    int rc = check_norm(a->T, a->H, a->dtype, a->w_dtype);
+    if (rc != MOE_OK || a->T == 0) return rc;
+    if ((rc = check_rows("x", a->x, a->x_stride, a->H)) != MOE_OK) return rc;
+    if (a->residual && (rc = check_rows("residual", a->residual, a->residual_stride, a->H)) != MOE_OK) return rc;
+    if (!a->weight || !a->q || !a->scales || !a->rstd || (a->residual && !a->h))
+        return fail(MOE_ERR_INVALID, "weight, q, scales, rstd (and h, with a residual) must be non-NULL");
+    if (!aligned16(a->weight) || !aligned16(a->q) || !aligned16(a->h) || !aligned16(a->y))
+        return fail(MOE_ERR_INVALID, "weight, q, h and y must be 16-byte aligned");
+    NormParams p;
+    p.x = a->x; p.x_stride = a->x_stride; p.residual = a->residual; p.res_stride = a->residual_stride;
+    p.weight = a->weight; p.q = static_cast<uint8_t*>(a->q); p.scales = a->scales; p.ss_row = a->ss_row; p.ss_blk = a->ss_blk;
+    p.h = a->h; p.y = a->y; p.rstd = a->rstd; p.T = a->T; p.H = a->H; p.eps = a->eps; p.pow2 = a->pow2 ? 1 : 0;
+    const NormShape s = norm_shape(a->H);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    with_dtype(a->dtype, [&](auto t) {
+        using T = decltype(t);
+        if (a->w_dtype == a->dtype) launch_norm<T, T>(p, s, st);
+        else launch_norm<T, float>(p, s, st);
+    });
+    CUDA_TRY(cudaGetLastError());
+    return MOE_OK;
+}
+
+size_t moe_rms_norm_backward_workspace_bytes(int32_t T, int32_t H) {
+    if (T < 0 || H <= 0) return 0;
+    return align256((size_t)(T < NORM_GRAD_MAX_PARTS ? (T > 0 ? T : 1) : NORM_GRAD_MAX_PARTS) * (size_t)H * 4);
+}
+
+int moe_rms_norm_backward(const moe_norm_grad_args* a, void* stream) {
+    if (!a) return fail(MOE_ERR_INVALID, "args is NULL");
+    int rc = check_norm(a->T, a->H, a->dtype, a->w_dtype);
+    if (rc != MOE_OK) return rc;
+    if (!a->dw || !aligned16(a->dw)) return fail(MOE_ERR_INVALID, "dw must be non-NULL and 16-byte aligned");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (a->T == 0) {
+        CUDA_TRY(cudaMemsetAsync(a->dw, 0, (size_t)a->H * 4, st));
+        return MOE_OK;
+    }
+    if ((rc = check_rows("dy", a->dy, a->dy_stride, a->H)) != MOE_OK) return rc;
+    if ((rc = check_rows("h", a->h, a->h_stride, a->H)) != MOE_OK) return rc;
+    if (a->dh && (rc = check_rows("dh", a->dh, a->dh_stride, a->H)) != MOE_OK) return rc;
+    if (!a->weight || !a->rstd || !a->dx || !aligned16(a->weight) || !aligned16(a->dx))
+        return fail(MOE_ERR_INVALID, "weight, rstd and dx must be non-NULL, weight and dx 16-byte aligned");
+    if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < moe_rms_norm_backward_workspace_bytes(a->T, a->H))
+        return fail(MOE_ERR_INVALID, "workspace too small or not 16-byte aligned (moe_rms_norm_backward_workspace_bytes)");
+    DeviceInfo* di = nullptr;
+    if ((rc = device_info(&di)) != MOE_OK) return rc;
+    NormGradParams p;
+    p.dy = a->dy; p.dy_stride = a->dy_stride; p.h = a->h; p.h_stride = a->h_stride; p.weight = a->weight; p.rstd = a->rstd;
+    p.dh = a->dh; p.dh_stride = a->dh_stride; p.dx = a->dx; p.partial = static_cast<float*>(a->workspace); p.T = a->T; p.H = a->H;
+    const NormShape s = norm_shape(a->H);
+    int grid = 2 * di->num_sms;
+    if (grid > NORM_GRAD_MAX_PARTS) grid = NORM_GRAD_MAX_PARTS;
+    if (grid > a->T) grid = a->T;
+    with_dtype(a->dtype, [&](auto t) {
+        using T = decltype(t);
+        if (a->w_dtype == a->dtype) launch_norm_grad<T, T>(p, grid, s, st);
+        else launch_norm_grad<T, float>(p, grid, s, st);
+    });
+    CUDA_TRY(cudaGetLastError());
+    rms_norm_dw_kernel<<<(a->H + 31) / 32, 1024, 0, st>>>(p.partial, a->dw, grid, a->H);
+    CUDA_TRY(cudaGetLastError());
+    return MOE_OK;
+}
+
+int moe_route(const moe_route_args* a, void* stream) {
+    if (!a) return fail(MOE_ERR_INVALID, "args is NULL");
+    int rc = check_route(a->T, a->E, a->top_k, a->dtype, a->score, a->stride);
+    if (rc != MOE_OK) return rc;
+    if (a->n_group <= 0 || a->n_group > RT_MAX_GROUPS || a->E % a->n_group)
+        return fail(MOE_ERR_INVALID, "n_group=%d must be in [1, %d] and divide E=%d", a->n_group, RT_MAX_GROUPS, a->E);
+    if (a->topk_group <= 0 || a->topk_group > a->n_group) return fail(MOE_ERR_INVALID, "topk_group must be in [1, n_group]");
+    if ((int64_t)a->topk_group * (a->E / a->n_group) < a->top_k) return fail(MOE_ERR_INVALID, "the kept groups hold fewer than top_k=%d experts", a->top_k);
+    if (a->group_score != MOE_GROUP_MAX && a->group_score != MOE_GROUP_TOP2) return fail(MOE_ERR_INVALID, "group_score must be MOE_GROUP_MAX or MOE_GROUP_TOP2");
+    if (a->bias && a->bias_dtype != MOE_DTYPE_BF16 && a->bias_dtype != MOE_DTYPE_F32) return fail(MOE_ERR_INVALID, "bias_dtype must be bf16 or f32");
+    if (a->T == 0) return MOE_OK;
+    if (!a->logits || !a->ids || !a->weights) return fail(MOE_ERR_INVALID, "logits, ids and weights must be non-NULL");
+    RouteParams p;
+    p.logits = a->logits; p.stride = a->stride; p.bias = a->bias; p.bias_bf16 = a->bias_dtype == MOE_DTYPE_BF16;
+    p.ids = a->ids; p.weights = a->weights; p.T = a->T; p.E = a->E; p.top_k = a->top_k; p.n_group = a->n_group;
+    p.topk_group = a->topk_group; p.sigmoid = a->score == MOE_SCORE_SIGMOID; p.top2 = a->group_score == MOE_GROUP_TOP2;
+    p.renorm = a->renormalize ? 1 : 0; p.vec = route_vec(a->logits, a->stride, a->E, a->dtype); p.scale = a->scale;
+    const size_t smem = a->bias || a->n_group > 1 ? (size_t)RT_WARPS * (a->E + RT_MAX_GROUPS) * 8 : 0;
+    with_dtype(a->dtype, [&](auto t) { launch_route<decltype(t)>(p, smem, static_cast<cudaStream_t>(stream)); });
+    CUDA_TRY(cudaGetLastError());
+    return MOE_OK;
+}
+
+int moe_route_backward(const moe_route_grad_args* a, void* stream) {
+    if (!a) return fail(MOE_ERR_INVALID, "args is NULL");
+    int rc = check_route(a->T, a->E, a->top_k, a->dtype, a->score, a->stride);
+    if (rc != MOE_OK || a->T == 0) return rc;
+    if (!a->grad_weights || !a->logits || !a->ids || !a->dlogits) return fail(MOE_ERR_INVALID, "grad_weights, logits, ids and dlogits must be non-NULL");
+    RouteGradParams p;
+    p.grad = a->grad_weights; p.logits = a->logits; p.stride = a->stride; p.ids = a->ids; p.out = a->dlogits;
+    p.T = a->T; p.E = a->E; p.top_k = a->top_k; p.sigmoid = a->score == MOE_SCORE_SIGMOID; p.renorm = a->renormalize ? 1 : 0;
+    p.vec = route_vec(a->logits, a->stride, a->E, a->dtype) && aligned16(a->dlogits); p.scale = a->scale;
+    with_dtype(a->dtype, [&](auto t) { launch_route_grad<decltype(t)>(p, static_cast<cudaStream_t>(stream)); });
+    CUDA_TRY(cudaGetLastError());
+    return MOE_OK;
+}
+
+int moe_quant_fp4(const moe_fp4_quant_args* a, void* stream) {
+    if (!a) return fail(MOE_ERR_INVALID, "args is NULL");
+    if (a->groups <= 0 || a->groups > 65535 || a->rows < 0 || a->src_rows < 0 || a->K <= 0 || a->K % 128)
+        return fail(MOE_ERR_INVALID, "groups must be in [1, 65535], rows non-negative and K=%d a positive multiple of 128", a->K);
+    if (a->format != MOE_FP4_NV && a->format != MOE_FP4_MX) return fail(MOE_ERR_INVALID, "format must be MOE_FP4_NV or MOE_FP4_MX");
+    if (!float_dtype(a->dtype)) return fail(MOE_ERR_INVALID, "dtype must be bf16, f16 or f32");
+    if (a->src_pair ? a->groups != 1 || a->top_k <= 0 : a->rows != a->src_rows)
+        return fail(MOE_ERR_INVALID, "src_pair needs one group and a positive top_k; without it rows and src_rows are the same");
+    if (a->factor && a->format == MOE_FP4_MX) return fail(MOE_ERR_INVALID, "mxfp4 has no factor");
+    if (a->rows == 0) return MOE_OK;
+    if (!a->q || !a->scales || (!a->x && a->src_rows > 0)) return fail(MOE_ERR_INVALID, "x, q and scales must be non-NULL");
+    const int64_t cols = a->silu_mul ? 2ll * a->K : a->K;
+    if (!aligned16(a->x) || a->x_stride < cols || a->x_stride % 8) return fail(MOE_ERR_INVALID, "x must be 16-byte aligned with a row stride that covers its columns and is a multiple of 8");
+    if (!aligned16(a->q) || !aligned16(a->scales)) return fail(MOE_ERR_INVALID, "q and scales must be 16-byte aligned");
+    Fp4QuantParams p;
+    p.x = a->x; p.x_stride = a->x_stride; p.factor = a->factor; p.factor_stride = a->factor_stride; p.src = a->src_pair; p.top_k = a->top_k;
+    p.q = static_cast<uint8_t*>(a->q); p.sf = static_cast<uint8_t*>(a->scales); p.rows = a->rows; p.K = a->K;
+    p.gate_first = a->gate_first ? 1 : 0; p.src_rows = a->src_rows; p.k_blocks = (a->K + 255) / 256;
+    const long long blocks = (long long)((a->rows + 127) / 128) * p.k_blocks;
+    if (blocks > 0x7FFFFFFFll) return fail(MOE_ERR_INVALID, "rows x K exceeds what one call covers");
+    const dim3 grid((unsigned)blocks, a->groups, 1);
+    with_dtype(a->dtype, [&](auto t) {
+        launch_quant_fp4<decltype(t)>(p, a->format == MOE_FP4_NV, a->silu_mul != 0, grid, static_cast<cudaStream_t>(stream));
+    });
+    CUDA_TRY(cudaGetLastError());
+    return MOE_OK;
+}
+
+int moe_unpack_fp4(const void* q, void* out_e4m3, int64_t n_bytes, void* stream) {
+    if (n_bytes < 0 || n_bytes % 8) return fail(MOE_ERR_INVALID, "n_bytes must be a non-negative multiple of 8");
+    if (n_bytes == 0) return MOE_OK;
+    if (!q || !out_e4m3 || !aligned16(q) || !aligned16(out_e4m3)) return fail(MOE_ERR_INVALID, "q and out must be non-NULL and 16-byte aligned");
+    const long long n = n_bytes / 8, blocks = (n + 255) / 256;
+    if (blocks > 0x7FFFFFFFll) return fail(MOE_ERR_INVALID, "n_bytes exceeds what one call covers");
+    unpack_fp4_kernel<<<(unsigned)blocks, 256, 0, static_cast<cudaStream_t>(stream)>>>(static_cast<const uint2*>(q), static_cast<uint4*>(out_e4m3), n);
+    CUDA_TRY(cudaGetLastError());
+    return MOE_OK;
+}
+
+int moe_gg_fp4_contiguous(const moe_gg_fp4_args* args, void* stream) { return launch_gg_fp4(args, false, stream); }
+int moe_gg_fp4_masked(const moe_gg_fp4_args* args, void* stream) { return launch_gg_fp4(args, true, stream); }
+
+}  // extern "C"

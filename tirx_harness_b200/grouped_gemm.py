@@ -16,7 +16,7 @@ import ctypes
 
 import torch
 
-from . import _lib
+from . import _lib, moe_ops
 
 
 def _ptr(t: torch.Tensor) -> int:
@@ -234,6 +234,80 @@ def bind_k_grouped(a, sfa_words, b, sfb_words, d, ks) -> _BoundKGrouped:
     MN-major, group g owns ``ks[g]`` consecutive K rows (multiples of 128), packed UE8M0 scales int32
     [sum(ceil(ks/512)), M] / [.., N], ``d`` f32 [G, M, N].  Returns the zero-argument callable."""
     return _BoundKGrouped(a, sfa_words, b, sfb_words, d, ks)
+
+
+class _BoundFp4:
+    """4-bit grouped GEMM bound to its tensors; ``__call__`` launches on the current stream of their device."""
+
+    def __init__(self, fn_name, a, sfa, b, sfb, d, layout, alpha, fmt, G, M, N, K, rows_used=None):
+        self._keep = (a, sfa, b, sfb, d, layout, alpha, rows_used)
+        self._fn = getattr(_lib.lib(), fn_name)
+        self._device = d.device
+        self._args = _lib.GGFp4Args(
+            a=_ptr(a), sfa=_ptr(sfa), b=_ptr(b), sfb=_ptr(sfb), alpha=_ptr(alpha) if alpha is not None else None,
+            alpha_stride=1 if alpha is not None and alpha.numel() > 1 else 0, layout=_ptr(layout),
+            rows_used=_ptr(rows_used) if rows_used is not None else None, d=_ptr(d), ldd=max(d.stride(-2), N), G=G, M=M, N=N, K=K,
+            format=moe_ops._FP4_FORMAT[fmt], d_dtype=1 if d.dtype == torch.float32 else 0)
+        self.out = d
+
+    def __call__(self):
+        with torch.cuda.device(self._device):
+            stream = torch.cuda.current_stream().cuda_stream
+            _lib.check(self._fn(ctypes.byref(self._args), ctypes.c_void_p(stream)))
+        return self.out
+
+
+def _check_fp4(a, sfa, b, sfb, layout, alpha, fmt, a_lead):
+    """Checks what both layouts share; -> (G, N, K).  a is [*a_lead, K/2]."""
+    moe_ops._choice(moe_ops.FP4_BLOCK, fmt, "fmt")
+    if b.dim() != 3 or b.dtype != torch.uint8 or not b.is_cuda or not b.is_contiguous():
+        raise ValueError("b must be contiguous uint8 [G, N, K/2] on a CUDA device")
+    G, N, K = b.shape[0], b.shape[1], 2 * b.shape[2]
+    if G == 0 or N == 0 or N % 8 or K == 0 or K % 128:
+        raise ValueError(f"G must be positive, N={N} a multiple of 8 and K={K} of 128")
+    dev = b.device
+    moe_ops._check_like(a, "a", (*a_lead, K // 2), torch.uint8, dev)
+    moe_ops._check_like(sfb, "sfb", (G, *moe_ops.fp4_scale_shape(N, K, fmt)), torch.uint8, dev)
+    lead = a_lead[:-1]
+    moe_ops._check_like(sfa, "sfa", (*lead, *moe_ops.fp4_scale_shape(a_lead[-1], K, fmt)), torch.uint8, dev)
+    if alpha is not None:
+        if alpha.numel() not in (1, G):
+            raise ValueError(f"alpha must hold one value or {G}")
+        moe_ops._check_like(alpha, "alpha", alpha.shape, torch.float32, dev)
+    if layout.dtype != torch.int32 or layout.device != dev or not layout.is_contiguous():
+        raise ValueError(f"the layout must be a contiguous int32 tensor on {dev}")
+    return G, N, K
+
+
+def bind_contiguous_fp4(a, sfa, b, sfb, d, grouped_layout, alpha=None, fmt: str = "nvfp4", rows_used=None) -> _BoundFp4:
+    """D[r] = alpha[g] * deq(a[r]) @ deq(b[g]).T for the rows r of group g = grouped_layout[r], 4-bit operands.
+
+    a uint8 [M, K/2], b uint8 [G, N, K/2] and their scale tiles sfa, sfb as :func:`moe_ops.quant_fp4` makes them (``fmt``);
+    d bf16 (or f32) [M, N]; alpha f32, one value or [G] (nvfp4: the product of the operands' global scales; default 1);
+    grouped_layout int32 [M], negative = padding row, left as it is; rows_used int32 [1] on the device."""
+    M = a.shape[0]
+    G, N, K = _check_fp4(a, sfa, b, sfb, grouped_layout, alpha, fmt, (M,))
+    if d.dtype not in (torch.bfloat16, torch.float32) or tuple(d.shape) != (M, N) or d.stride(1) != 1 or d.device != b.device:
+        raise ValueError(f"d must be bfloat16 (or float32) [{M}, {N}] with unit column stride on {b.device}")
+    if grouped_layout.numel() != M:
+        raise ValueError(f"grouped_layout must be int32 [{M}]")
+    if rows_used is not None and (rows_used.dtype != torch.int32 or rows_used.device != b.device):
+        raise ValueError(f"rows_used must be an int32 tensor on {b.device}")
+    return _BoundFp4("moe_gg_fp4_contiguous", a, sfa, b, sfb, d, grouped_layout, alpha, fmt, G, M, N, K, rows_used)
+
+
+def bind_masked_fp4(a, sfa, b, sfb, d, masked_m, alpha=None, fmt: str = "nvfp4") -> _BoundFp4:
+    """The same for the masked layout: a uint8 [G, max_m, K/2] with a group's own scale tiles, d [G, max_m, N], of which
+    the first masked_m[g] rows of each group are computed and the others left as they are."""
+    if a.dim() != 3:
+        raise ValueError("a must be uint8 [G, max_m, K/2]")
+    M = a.shape[1]
+    G, N, K = _check_fp4(a, sfa, b, sfb, masked_m, alpha, fmt, (a.shape[0], M))
+    if a.shape[0] != G or masked_m.numel() != G:
+        raise ValueError(f"a and masked_m must have {G} groups")
+    if d.dtype not in (torch.bfloat16, torch.float32) or tuple(d.shape) != (G, M, N) or not d.is_contiguous() or d.device != b.device:
+        raise ValueError(f"d must be contiguous bfloat16 (or float32) [{G}, {M}, {N}] on {b.device}")
+    return _BoundFp4("moe_gg_fp4_masked", a, sfa, b, sfb, d, masked_m, alpha, fmt, G, M, N, K)
 
 
 def m_grouped_fp8_gemm_nt_contiguous(a, sfa, b, sfb, d, grouped_layout):

@@ -129,3 +129,241 @@ def combine(y: torch.Tensor, pos: torch.Tensor, w: torch.Tensor, out=None):
         _lib.check(_lib.lib().moe_combine(_vp(y.data_ptr()), _vp(pos.data_ptr()), _vp(w.data_ptr()), _vp(out.data_ptr()),
                                           _i32(T), _i32(top_k), _i32(H), _stream(y)))
     return out
+
+
+# ------------------------------------------------------------------ norm, routing and 4-bit operands
+_DTYPE = {torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32, torch.float16: _lib.DTYPE_F16}
+FP4_BLOCK = {"nvfp4": 16, "mxfp4": 32}           # values under one scale
+_FP4_FORMAT = {"nvfp4": _lib.FP4_NV, "mxfp4": _lib.FP4_MX}
+
+
+def _p(t):
+    return t.data_ptr() if t is not None else None
+
+
+def _check_float(t, name, dtypes=tuple(_DTYPE)):
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} must be one of {', '.join(str(d)[6:] for d in dtypes)}, got {t.dtype}")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+
+
+def _check_like(t, name, shape, dtype, device, contiguous=True):
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the other tensors on {device}")
+    if contiguous and not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _row_stride(t, name):
+    """Elements between the rows of a 2-d tensor whose columns are next to one another."""
+    if t.dim() != 2:
+        raise ValueError(f"{name} must have two dimensions, got {t.dim()}")
+    if t.shape[1] != 1 and t.stride(1) != 1:
+        raise ValueError(f"{name} must have unit column stride")
+    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], t.stride(0) // 8 * 8)
+
+
+def _launch(fn_name, args, device):
+    with torch.cuda.device(device):
+        _lib.check(getattr(_lib.lib(), fn_name)(ctypes.byref(args), _vp(torch.cuda.current_stream(device).cuda_stream)))
+
+
+def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-6,
+                   pow2: bool = False, mn_major: bool = False, want_y: bool = False):
+    """Residual addition, root-mean-square norm and 1x128 quantisation in one pass.
+
+    x, residual bf16/f16/f32 [T, H] (any row stride that is a multiple of 8), weight [H] of x's type or f32 ->
+    dict(q e4m3 [T, H], scales f32 [T, ceil(H/128)], h, y, rstd f32 [T]) with h = round(x + residual) (x itself without a
+    residual), y = h * rstd * weight (x's type; None unless ``want_y``) and q, scales its 1x128 quantisation as
+    :func:`quant_1x128` does it, from y in fp32.  ``pow2`` rounds the scales up to powers of two, which the grouped GEMM
+    applies inside the tensor core; ``mn_major`` stores them [H/128, T].  H % 8 == 0, H <= 16384."""
+    _check_float(x, "x")
+    ld = _row_stride(x, "x")
+    T, H = x.shape
+    if weight.dtype not in (x.dtype, torch.float32):
+        raise TypeError(f"weight must be {x.dtype} or float32, got {weight.dtype}")
+    _check_like(weight, "weight", (H,), weight.dtype, x.device)
+    ldr = 0
+    if residual is not None:
+        _check_like(residual, "residual", (T, H), x.dtype, x.device, contiguous=False)
+        ldr = _row_stride(residual, "residual")
+    q = torch.empty((T, H), dtype=torch.float8_e4m3fn, device=x.device)
+    s = _scale_out(T, (H + 127) // 128, mn_major, x.device)
+    h = torch.empty((T, H), dtype=x.dtype, device=x.device) if residual is not None else x
+    y = torch.empty((T, H), dtype=x.dtype, device=x.device) if want_y else None
+    rstd = torch.empty(T, dtype=torch.float32, device=x.device)
+    _launch("moe_rms_norm_quant", _lib.NormArgs(
+        x=_p(x), x_stride=ld, residual=_p(residual), residual_stride=ldr, weight=_p(weight), q=_p(q), scales=_p(s),
+        ss_row=s.stride(0), ss_blk=s.stride(1), h=_p(h) if residual is not None else None, y=_p(y), rstd=_p(rstd), T=T, H=H,
+        dtype=_DTYPE[x.dtype], w_dtype=_DTYPE[weight.dtype], pow2=1 if pow2 else 0, eps=eps), x.device)
+    return dict(q=q, scales=s, h=h, y=y, rstd=rstd)
+
+
+def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor,
+                      dh: torch.Tensor | None = None):
+    """Gradient of :func:`rms_norm_quant`, the rounding to 8 bits passed through unchanged.
+
+    dy = dL/dy and h [T, H] of one type, rstd from the forward call, dh (optional) the gradient that reaches h past the
+    norm -> (dx [T, H], the gradient of x and of residual alike; dw f32 [H])."""
+    _check_float(dy, "dy")
+    ld = _row_stride(dy, "dy")
+    T, H = dy.shape
+    _check_like(h, "h", (T, H), dy.dtype, dy.device, contiguous=False)
+    if weight.dtype not in (dy.dtype, torch.float32):
+        raise TypeError(f"weight must be {dy.dtype} or float32, got {weight.dtype}")
+    _check_like(weight, "weight", (H,), weight.dtype, dy.device)
+    _check_like(rstd, "rstd", (T,), torch.float32, dy.device)
+    ldd = 0
+    if dh is not None:
+        _check_like(dh, "dh", (T, H), dy.dtype, dy.device, contiguous=False)
+        ldd = _row_stride(dh, "dh")
+    dx = torch.empty((T, H), dtype=dy.dtype, device=dy.device)
+    dw = torch.empty(H, dtype=torch.float32, device=dy.device)
+    n = _lib.lib().moe_rms_norm_backward_workspace_bytes(_i32(T), _i32(H))
+    ws = torch.empty(n, dtype=torch.uint8, device=dy.device)
+    _launch("moe_rms_norm_backward", _lib.NormGradArgs(
+        dy=_p(dy), dy_stride=ld, h=_p(h), h_stride=_row_stride(h, "h"), weight=_p(weight), rstd=_p(rstd), dh=_p(dh), dh_stride=ldd,
+        dx=_p(dx), dw=_p(dw), T=T, H=H, dtype=_DTYPE[dy.dtype], w_dtype=_DTYPE[weight.dtype], workspace=_p(ws), workspace_bytes=n),
+        dy.device)
+    return dx, dw
+
+
+_SCORE = {"softmax": 0, "sigmoid": 1}
+_GROUP_SCORE = {"max": 0, "top2": 1}
+
+
+def _choice(table, value, name):
+    if value not in table:
+        raise ValueError(f"{name} must be one of {', '.join(table)}, got {value!r}")
+    return table[value]
+
+
+def route(logits: torch.Tensor, top_k: int, score: str = "softmax", bias: torch.Tensor | None = None, n_group: int = 1,
+          topk_group: int = 1, group_score: str = "top2", renormalize: bool = True, scale: float = 1.0):
+    """Top-k routing: bf16/f16/f32 [T, E] -> (ids int32 [T, top_k], weights f32 [T, top_k]).
+
+    p = softmax or sigmoid of the logits; the experts are chosen by p + bias (bf16/f32 [E]) in its exact order, ties to the
+    lowest index, and weighted by p (over its sum of the chosen with ``renormalize``) * scale.  With n_group > 1 only the
+    topk_group best groups of E / n_group consecutive experts count; a group's score is its best p + bias ("max") or the
+    sum of its two best ("top2").  A logit of -inf or NaN switches its expert off; where fewer than top_k are left the id
+    is -1 and the weight 0, which :func:`permute_plan` drops."""
+    _check_float(logits, "logits")
+    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError("logits must be [T, E] with unit column stride")
+    T, E = logits.shape
+    if bias is not None:
+        _check_float(bias, "bias", (torch.bfloat16, torch.float32))
+        _check_like(bias, "bias", (E,), bias.dtype, logits.device)
+    if not 0 < top_k <= min(32, E):
+        raise ValueError(f"top_k must be in [1, min(32, E)], got {top_k}")
+    ids = torch.empty((T, top_k), dtype=torch.int32, device=logits.device)
+    w = torch.empty((T, top_k), dtype=torch.float32, device=logits.device)
+    _launch("moe_route", _lib.RouteArgs(
+        logits=_p(logits), stride=max(logits.stride(0), E) if T < 2 else logits.stride(0), bias=_p(bias), ids=_p(ids), weights=_p(w),
+        T=T, E=E, top_k=top_k, n_group=n_group, topk_group=topk_group, dtype=_DTYPE[logits.dtype],
+        bias_dtype=_DTYPE[bias.dtype] if bias is not None else 0, score=_choice(_SCORE, score, "score"),
+        group_score=_choice(_GROUP_SCORE, group_score, "group_score"), renormalize=1 if renormalize else 0, scale=scale), logits.device)
+    return ids, w
+
+
+def route_backward(grad_weights: torch.Tensor, logits: torch.Tensor, ids: torch.Tensor, score: str = "softmax",
+                   renormalize: bool = True, scale: float = 1.0):
+    """Gradient of :func:`route`'s weights with respect to the logits, the choice held fixed: [T, E] of the logits' type."""
+    _check_float(logits, "logits")
+    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError("logits must be [T, E] with unit column stride")
+    T, E = logits.shape
+    if ids.dim() != 2:
+        raise ValueError("ids must be [T, top_k]")
+    top_k = ids.shape[1]
+    _check_like(ids, "ids", (T, top_k), torch.int32, logits.device)
+    _check_like(grad_weights, "grad_weights", (T, top_k), torch.float32, logits.device)
+    out = torch.empty((T, E), dtype=logits.dtype, device=logits.device)
+    _launch("moe_route_backward", _lib.RouteGradArgs(
+        grad_weights=_p(grad_weights), logits=_p(logits), stride=max(logits.stride(0), E) if T < 2 else logits.stride(0), ids=_p(ids),
+        dlogits=_p(out), T=T, E=E, top_k=top_k, dtype=_DTYPE[logits.dtype], score=_choice(_SCORE, score, "score"),
+        renormalize=1 if renormalize else 0, scale=scale), logits.device)
+    return out
+
+
+def fp4_scale_shape(rows: int, K: int, fmt: str = "nvfp4"):
+    """Shape of the scale tiles of ``rows`` x K values: uint8 [ceil(rows/128), ceil(K/256) * (4 nvfp4, 2 mxfp4), 512];
+    row r's bytes of a tile's four blocks are at (r % 32) * 16 + (r // 32 % 4) * 4."""
+    return ((rows + 127) // 128, (K + 255) // 256 * (64 // _choice(FP4_BLOCK, fmt, "fmt")), 512)
+
+
+def quant_fp4(x: torch.Tensor, fmt: str = "nvfp4", global_scale: torch.Tensor | None = None, act: str | None = None,
+              gate_first: bool = True, src_pair: torch.Tensor | None = None, top_k: int = 1, out=None):
+    """Quantises to 4-bit blocks: -> (codes uint8 [.., rows, K/2], scale tiles uint8 [.., *fp4_scale_shape(rows, K, fmt)]).
+
+    x bf16/f16/f32 [rows, K] (row stride a multiple of 8) or, for operands of several groups, contiguous [G, rows, K].
+      fmt          "nvfp4": one e4m3 scale per 16 values under ``global_scale`` (f32, one value or [G]; default 1):
+                   s = e4m3(min(amax / (6 g), 448)), value = code * s * g.  "mxfp4": a power of two per 32 values
+      act          "silu_mul": x is [rows, 2K] and SiLU(gate) * up, in fp32, is quantised (gate = the first half, or the
+                   second with gate_first=False)
+      src_pair     int32 [rows]: row r is made from x[src_pair[r] // top_k], as :func:`permute` gathers; where it is negative
+                   the row of ``out`` is left as it is
+      out          (codes, scales) to write into; without it codes and scales of skipped rows are zero
+    K % 128 == 0.  A block that holds an infinity or a NaN gets the scale NaN."""
+    _check_float(x, "x")
+    block = _choice(FP4_BLOCK, fmt, "fmt")
+    if act not in (None, "silu_mul"):
+        raise ValueError(f"act must be None or 'silu_mul', got {act!r}")
+    if x.dim() == 3:
+        if not x.is_contiguous():
+            raise ValueError("a three-dimensional x must be contiguous")
+        G, src_rows, cols = x.shape
+        ld, lead = cols, (G,)
+    else:
+        ld, (src_rows, cols), G, lead = _row_stride(x, "x"), x.shape, 1, ()
+    if act is not None and cols % 2:
+        raise ValueError("with act='silu_mul' x must be [rows, 2K]")
+    K = cols // 2 if act is not None else cols
+    if K == 0 or K % 128:
+        raise ValueError(f"K={K} must be a positive multiple of 128")
+    rows = src_rows
+    if src_pair is not None:
+        if G != 1 or x.dim() == 3:
+            raise ValueError("src_pair needs a two-dimensional x")
+        _check_like(src_pair, "src_pair", (src_pair.numel(),), torch.int32, x.device)
+        if top_k < 1:
+            raise ValueError("top_k must be positive")
+        rows = src_pair.numel()
+    gs = 0
+    if global_scale is not None:
+        if fmt != "nvfp4":
+            raise ValueError("global_scale belongs to nvfp4")
+        if global_scale.numel() not in (1, G):
+            raise ValueError(f"global_scale must hold one value or {G}")
+        _check_like(global_scale, "global_scale", global_scale.shape, torch.float32, x.device)
+        gs = 1 if global_scale.numel() > 1 else 0
+    q_shape, s_shape = (*lead, rows, K // 2), (*lead, *fp4_scale_shape(rows, K, fmt))
+    if out is not None:
+        q, s = out
+        _check_like(q, "out[0]", q_shape, torch.uint8, x.device)
+        _check_like(s, "out[1]", s_shape, torch.uint8, x.device)
+    else:
+        make = torch.empty if src_pair is None else torch.zeros
+        q, s = make(q_shape, dtype=torch.uint8, device=x.device), make(s_shape, dtype=torch.uint8, device=x.device)
+    if G == 0 or rows == 0:
+        return q, s
+    _launch("moe_quant_fp4", _lib.Fp4QuantArgs(
+        x=_p(x), x_stride=ld, factor=_p(global_scale), factor_stride=gs, src_pair=_p(src_pair), q=_p(q), scales=_p(s), groups=G,
+        rows=rows, src_rows=src_rows, K=K, top_k=top_k, dtype=_DTYPE[x.dtype], format=_FP4_FORMAT[fmt],
+        silu_mul=1 if act is not None else 0, gate_first=1 if gate_first else 0), x.device)
+    return q, s
+
+
+def unpack_fp4(q: torch.Tensor):
+    """Packed codes uint8 [.., K/2] -> their values as e4m3 [.., K] (every e2m1 value is one)."""
+    if q.dtype != torch.uint8 or not q.is_cuda or not q.is_contiguous() or q.dim() == 0 or q.shape[-1] % 8:
+        raise ValueError("q must be a contiguous uint8 CUDA tensor whose last dimension is a multiple of 8")
+    out = torch.empty((*q.shape[:-1], 2 * q.shape[-1]), dtype=torch.float8_e4m3fn, device=q.device)
+    with torch.cuda.device(q.device):
+        _lib.check(_lib.lib().moe_unpack_fp4(_vp(q.data_ptr()), _vp(out.data_ptr()), _i64(q.numel()), _stream(q)))
+    return out
