@@ -92,6 +92,47 @@ void launch_quant_fp4(const Fp4QuantParams& p, bool nv, bool silu, dim3 grid, cu
     else quant_fp4_kernel<T, false, false><<<grid, FP4_QUANT_THREADS, 0, st>>>(p);
 }
 
+// 1-D array of scale tiles as 64-bit words, box = one chunk (the scales of 128 rows x 256 values)
+int encode_scale_chunks(CUtensorMap* map, const void* base, uint64_t bytes, uint32_t chunk) {
+    auto fn = get_encode_fn();
+    if (!fn) return fail(MOE_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+    cuuint64_t dims[1] = {bytes / 8};
+    cuuint64_t strides[1] = {0};
+    cuuint32_t box[1] = {chunk / 8};
+    cuuint32_t estr[1] = {1};
+    CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT64, 1, const_cast<void*>(base), dims, strides, box, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(MOE_ERR_CUDA, "cuTensorMapEncodeTiled (scales) failed with CUresult %d", (int)r);
+    return MOE_OK;
+}
+
+template <bool NV, bool MASKED, int TN>
+int launch_fp4_pair(const GGFp4Params& p, long long rows_total, DeviceInfo* di, cudaStream_t st) {
+    using C = f4::Cfg<NV, TN>;
+    CUtensorMap ta, tb, tsa, tsb;
+    int rc;
+    const uint64_t kt = (uint64_t)p.kt * 512;
+    if ((rc = encode_fp8_kmajor(&ta, p.a, (uint64_t)rows_total, (uint64_t)p.K / 2, f4::BM)) != MOE_OK) return rc;
+    if ((rc = encode_fp8_kmajor(&tb, p.b, (uint64_t)p.G * p.N, (uint64_t)p.K / 2, TN / 2)) != MOE_OK) return rc;
+    if ((rc = encode_scale_chunks(&tsa, p.sfa, (uint64_t)(MASKED ? p.G : 1) * p.a_tiles * kt, C::SF_CHUNK)) != MOE_OK) return rc;
+    if ((rc = encode_scale_chunks(&tsb, p.sfb, (uint64_t)p.G * p.b_tiles * kt, C::SF_CHUNK)) != MOE_OK) return rc;
+    GGParams sp = {};
+    sp.layout = p.layout; sp.rows_used = p.rows_used; sp.G = p.G; sp.M = p.M; sp.N = p.N;
+    sp.num_n_blocks = (p.N + TN - 1) / TN;
+    const long long blocks = MASKED ? (long long)p.G * ((p.M + 255) / 256) : (p.M + 255) / 256;
+    const long long tiles = blocks * sp.num_n_blocks;
+    const int pairs = (int)(tiles < di->max_pairs ? tiles : di->max_pairs);
+    CUDA_TRY(cudaFuncSetAttribute((gg_fp4_pair_kernel<NV, MASKED, TN>), cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES));
+    gg_fp4_pair_kernel<NV, MASKED, TN><<<2 * pairs, f4::THREADS, C::SMEM_BYTES, st>>>(ta, tb, tsa, tsb, p, sp, di->status);
+    CUDA_TRY(cudaGetLastError());
+    return MOE_OK;
+}
+template <bool NV, int TN>
+int launch_fp4_pair_layout(const GGFp4Params& p, long long rows_total, DeviceInfo* di, cudaStream_t st) {
+    return p.masked ? launch_fp4_pair<NV, true, TN>(p, rows_total, di, st) : launch_fp4_pair<NV, false, TN>(p, rows_total, di, st);
+}
+
 int launch_gg_fp4(const moe_gg_fp4_args* a, bool masked, void* stream) {
     if (!a) return fail(MOE_ERR_INVALID, "args is NULL");
     if (a->G <= 0 || a->N <= 0 || a->K <= 0 || a->M < 0)
@@ -104,6 +145,8 @@ int launch_gg_fp4(const moe_gg_fp4_args* a, bool masked, void* stream) {
     if (masked && a->G > gg::MAX_MASKED_GROUPS) return fail(MOE_ERR_INVALID, "masked layout supports at most %d groups", gg::MAX_MASKED_GROUPS);
     const long long rows_total = masked ? (long long)a->G * a->M : (long long)a->M;
     if (rows_total > 0x7FFFFFFFll || (long long)a->G * a->N > 0x7FFFFFFFll) return fail(MOE_ERR_INVALID, "row counts exceed 2^31-1");
+    const long long chunks = (masked ? (long long)a->G : 1) * ((a->M + 127) / 128) + (long long)a->G * ((a->N + 127) / 128);
+    if (chunks * ((a->K + 255) / 256) > 0x7FFFFFFFll / 256) return fail(MOE_ERR_INVALID, "the scales exceed 2^31 64-bit words");
     if (a->alpha && a->alpha_stride != 0 && a->alpha_stride != 1) return fail(MOE_ERR_INVALID, "alpha_stride must be 0 or 1");
     if (rows_total == 0) return MOE_OK;
     if (!a->a || !a->sfa || !a->b || !a->sfb || !a->layout || !a->d) return fail(MOE_ERR_INVALID, "a, sfa, b, sfb, layout and d must all be non-NULL");
@@ -122,11 +165,7 @@ int launch_gg_fp4(const moe_gg_fp4_args* a, bool masked, void* stream) {
     p.kt = (a->K + 255) / 256 * (a->format == MOE_FP4_NV ? 4 : 2);
     p.a_tiles = (a->M + 127) / 128; p.b_tiles = (a->N + 127) / 128;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    dim3 grid((a->M + 63) / 64, (a->N + 63) / 64, masked ? a->G : 1);
-    if (a->format == MOE_FP4_NV) gg_fp4_simple_kernel<true><<<grid, 256, 0, st>>>(p);
-    else gg_fp4_simple_kernel<false><<<grid, 256, 0, st>>>(p);
-    CUDA_TRY(cudaGetLastError());
-    return MOE_OK;
+    return a->format == MOE_FP4_NV ? launch_fp4_pair_layout<true, 256>(p, rows_total, di, st) : launch_fp4_pair_layout<false, 256>(p, rows_total, di, st);
 }
 
 }  // namespace
