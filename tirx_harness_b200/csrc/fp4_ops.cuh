@@ -10,7 +10,7 @@
 // core takes them: tiles of 512 bytes for 128 rows x 4 blocks, row r's four bytes at (r % 32) * 16 + (r / 32) * 4; the
 // tiles of a row block follow one another along K, which is filled up to a multiple of 256 with zero scales.
 //
-// Bound by memory.  A block of threads takes 128 rows x 256 columns, so that the scales it makes are whole tiles.
+// Bound by memory: a thread holds the 16 columns of several rows at a time, so that enough loads are under way.
 #pragma once
 
 #include <cuda_fp4.h>
@@ -33,95 +33,146 @@ struct Fp4QuantParams {
 };
 
 // eight values -> eight codes, the first in the lowest four bits
-__device__ __forceinline__ uint32_t pack8_e2m1(const float* v) {
+__device__ __forceinline__ uint32_t pack8_e2m1(const f32x2 (&v)[4]) {
     uint32_t r = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        r |= (uint32_t)__nv_cvt_float2_to_fp4x2(make_float2(v[2 * i], v[2 * i + 1]), __NV_E2M1, cudaRoundNearest) << (8 * i);
+        r |= (uint32_t)__nv_cvt_float2_to_fp4x2(make_float2(lo2(v[i]), hi2(v[i])), __NV_E2M1, cudaRoundNearest) << (8 * i);
     return r;
 }
 
-constexpr int FP4_QUANT_THREADS = 256;
+// The largest magnitude of 16 values.  As unsigned numbers the magnitudes of a 16-bit type are in order, with infinity and
+// NaN above the others, and two of them are compared at a time.
+template <typename T> __device__ __forceinline__ float largest16(const Raw8<T>& a, const Raw8<T>& b) {
+    uint32_t m = 0;
+    const uint32_t u[8] = {a.w[0].x, a.w[0].y, a.w[0].z, a.w[0].w, b.w[0].x, b.w[0].y, b.w[0].z, b.w[0].w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = __vmaxu2(m, u[i] & 0x7FFF7FFFu);
+    m = max(m & 0xFFFFu, m >> 16);
+    return lo2(Fmt<T>::up(m));
+}
+template <> __device__ __forceinline__ float largest16<float>(const Raw8<float>& a, const Raw8<float>& b) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint4 w = i < 2 ? a.w[i & 1] : b.w[i & 1];
+        m = max(max(m, w.x & 0x7FFFFFFFu), max(w.y & 0x7FFFFFFFu, max(w.z & 0x7FFFFFFFu, w.w & 0x7FFFFFFFu)));
+    }
+    return __uint_as_float(m);
+}
+
+// x / (1 + exp(-x)) with the hardware's exp2 and reciprocal: off by less than 2^-20 of the value for |x| <= 20 (exp2 and
+// the rounding of its argument 2^-22 + |x| 2^-24 of 1 + exp, the reciprocal 2^-23), a thousandth of a 4-bit step.
+__device__ __forceinline__ float silu_quick(float x) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * -1.4426950408889634f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return x * r;
+}
+
+constexpr int FP4_QUANT_THREADS = 256, FP4_QUANT_ROWS = 64;
 
 // NV: nvfp4, else mxfp4.  SILU: x holds gate and up, K columns each.
-// A thread takes 16 columns of a row at a time (a block of nvfp4, half a block of mxfp4).
+// Block: 64 rows x 256 columns.  A thread takes 16 columns of a row at a time (a block of nvfp4, half a block of mxfp4) and
+// four such rows in all: of 16-bit inputs all four are loaded before the first is used, of the others two at a time.
 template <typename T, bool NV, bool SILU>
 __global__ void __launch_bounds__(FP4_QUANT_THREADS) quant_fp4_kernel(const Fp4QuantParams p) {
     constexpr int WORDS = NV ? 4 : 2;           // scale tiles of 256 columns
-    __shared__ uint32_t tile[WORDS * 128];
-    const int group = blockIdx.y, row_blocks = (p.rows + 127) >> 7;
+    constexpr int STEP = FP4_QUANT_THREADS / 16, ROWS = FP4_QUANT_ROWS / STEP, BATCH = sizeof(T) == 2 && !SILU ? ROWS : ROWS / 2;
+    __shared__ uint32_t tile[WORDS][FP4_QUANT_ROWS];
+    const int group = blockIdx.y, row_pieces = ((p.rows + 127) >> 7) * (128 / FP4_QUANT_ROWS);
     const int rb = blockIdx.x / p.k_blocks, kb = blockIdx.x - rb * p.k_blocks;
-    const int k0 = kb * 256, r0 = rb * 128;
-    const int seg = threadIdx.x & 15, col = k0 + seg * 16;
+    const int r0 = rb * FP4_QUANT_ROWS, i0 = threadIdx.x >> 4;
+    const int seg = threadIdx.x & 15, col = kb * 256 + seg * 16;
     const float g = p.factor ? __ldg(p.factor + group * p.factor_stride) : 1.0f;
-    const float g6 = __fmul_rn(6.0f, g);
-    uint8_t* tb = reinterpret_cast<uint8_t*>(tile);
-    const T* xg = static_cast<const T*>(p.x) + (long long)group * p.src_rows * p.x_stride;
-#pragma unroll 2
-    for (int i = threadIdx.x >> 4; i < 128; i += FP4_QUANT_THREADS / 16) {
-        const int r = r0 + i;
-        int s = r < p.rows ? r : -1;
-        if (s >= 0 && p.src) { s = __ldg(p.src + r); if (s >= 0) s /= p.top_k; }
-        const bool live = s >= 0 && s < p.src_rows && col < p.K;        // the same for all threads of a scale block
-        float v[16];
-        uint32_t amax = 0;
-        if (live) {
-            const T* row = xg + s * p.x_stride + col;
-            const Pack8<T> a = load8(row + (SILU && !p.gate_first ? p.K : 0)), b = load8(row + (SILU && !p.gate_first ? p.K : 0) + 8);
+    const float g6 = __fmul_rn(6.0f, g), r6 = __frcp_rn(g6);
+    const T* xg = static_cast<const T*>(p.x) + (long long)group * p.src_rows * p.x_stride + col;
+    const int gate = SILU && !p.gate_first ? p.K : 0, up = p.gate_first ? p.K : 0;
+    int src[ROWS];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) { v[j] = to_f32(a.v[j]); v[8 + j] = to_f32(b.v[j]); }
+    for (int k = 0; k < ROWS; ++k) {
+        const int r = r0 + i0 + k * STEP;
+        src[k] = r < p.rows && col < p.K ? (p.src ? __ldg(p.src + r) : r) : -1;
+    }
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+        if (p.src && src[k] >= 0) src[k] = src[k] / p.top_k;
+        if (src[k] >= p.src_rows) src[k] = -1;
+    }
+#pragma unroll
+    for (int b = 0; b < ROWS; b += BATCH) {
+        Raw8<T> x[BATCH][2], u[SILU ? BATCH : 1][2];
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+            if (src[b + k] < 0) continue;
+            const T* row = xg + src[b + k] * p.x_stride;
+            x[k][0] = load8(row + gate);
+            x[k][1] = load8(row + gate + 8);
             if (SILU) {
-                const Pack8<T> c = load8(row + (p.gate_first ? p.K : 0)), d = load8(row + (p.gate_first ? p.K : 0) + 8);
+                u[k][0] = load8(row + up);
+                u[k][1] = load8(row + up + 8);
+            }
+        }
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    v[j] = __fmul_rn(silu_f32(v[j]), to_f32(c.v[j]));
-                    v[8 + j] = __fmul_rn(silu_f32(v[8 + j]), to_f32(d.v[j]));
+        for (int k = 0; k < BATCH; ++k) {
+            const int i = i0 + (b + k) * STEP;
+            const bool live = src[b + k] >= 0;             // the same for all threads of a scale block
+            f32x2 v[2][4];
+            float amax = largest16(x[k][0], x[k][1]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                unpack8(x[k][h], v[h]);
+                if (SILU) {
+                    f32x2 w[4];
+                    unpack8(u[k][h], w);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[h][j] = mul2(pack_f32x2(silu_quick(lo2(v[h][j])), silu_quick(hi2(v[h][j]))), w[j]);
                 }
             }
+            if (SILU) {
+                amax = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) amax = max(amax, __float_as_uint(v[j]) & 0x7FFFFFFFu);
-        }
-        if (!NV) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        uint32_t byte = 0, lo = 0, hi = 0;
-        if (live) {
-            const bool finite = amax < 0x7F800000u;
-            if (NV) {
-                const float t = fminf(__fdiv_rn(__uint_as_float(amax), g6), 448.0f);
-                byte = finite ? __nv_cvt_float_to_fp8(t, __NV_SATFINITE, __NV_E4M3) : 0x7Fu;
-                const float unit = __fmul_rn(__half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3))), g);
-                if (finite && unit > 0.0f) {
-                    if (div_ok(unit)) {
-                        const float rc = __frcp_rn(unit);
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) v[j] = div_by(v[j], unit, rc);
+                for (int j = 0; j < 8; ++j) amax = amax_nan(amax_nan(amax, lo2(v[j >> 2][j & 3])), hi2(v[j >> 2][j & 3]));
+            }
+            if (!NV) amax = amax_nan(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+            uint32_t byte = 0;
+            if (live) {
+                const bool finite = amax < INFINITY;
+                if (NV) {
+                    // a quotient that overflows in div_by becomes NaN, which fminf takes for 448 too
+                    const float t = div_ok(g6) ? lo2(div_by(both(amax), both(-g6), both(r6))) : __fdiv_rn(amax, g6);
+                    byte = finite ? __nv_cvt_float_to_fp8(fminf(t, 448.0f), __NV_SATFINITE, __NV_E4M3) : 0x7Fu;
+                    const float unit = __fmul_rn(__half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3))), g);
+                    if (finite && unit > 0.0f) {
+                        div8(v[0], unit);
+                        div8(v[1], unit);
                     } else {
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) v[j] = __fdiv_rn(v[j], unit);
+                        for (int j = 0; j < 4; ++j) v[0][j] = v[1][j] = 0;
                     }
                 } else {
+                    byte = finite ? (uint32_t)max((int)(__float_as_uint(amax) >> 23) - 2, 0) : 0xFFu;
+                    const f32x2 inv = both(__uint_as_float((254u - byte) << 23));                 // 2^(127 - byte), exact
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) v[j] = 0.0f;
+                    for (int j = 0; j < 4; ++j) {
+                        v[0][j] = finite ? mul2(v[0][j], inv) : 0;
+                        v[1][j] = finite ? mul2(v[1][j], inv) : 0;
+                    }
                 }
-            } else {
-                const int e = (int)(amax >> 23) - 2;
-                byte = finite ? (uint32_t)max(e, 0) : 0xFFu;
-                const float inv = finite ? __uint_as_float((254u - byte) << 23) : 0.0f;         // 2^(127 - byte), exact
-#pragma unroll
-                for (int j = 0; j < 16; ++j) v[j] = finite ? __fmul_rn(v[j], inv) : 0.0f;
+                *reinterpret_cast<uint2*>(p.q + ((long long)group * p.rows + r0 + i) * (p.K >> 1) + (col >> 1)) =
+                    make_uint2(pack8_e2m1(v[0]), pack8_e2m1(v[1]));
             }
-            lo = pack8_e2m1(v);
-            hi = pack8_e2m1(v + 8);
-            *reinterpret_cast<uint2*>(p.q + ((long long)group * p.rows + r) * (p.K >> 1) + (col >> 1)) = make_uint2(lo, hi);
+            const int blk = NV ? seg : seg >> 1;            // block of these 256 columns
+            if (NV || !(seg & 1)) reinterpret_cast<uint8_t*>(&tile[blk >> 2][i])[blk & 3] = (uint8_t)byte;
         }
-        const int b = NV ? seg : seg >> 1;                  // block of these 256 columns
-        if (NV || !(seg & 1)) tb[(b >> 2) * 512 + (i & 31) * 16 + (i >> 5) * 4 + (b & 3)] = (uint8_t)byte;
     }
     __syncthreads();
-    uint32_t* out = reinterpret_cast<uint32_t*>(p.sf) + (((long long)group * row_blocks + rb) * p.k_blocks + kb) * (WORDS * 128);
-    for (int w = threadIdx.x; w < WORDS * 128; w += FP4_QUANT_THREADS) {
-        const int r = r0 + ((w & 127) >> 2) + (w & 3) * 32;
+    uint32_t* out = reinterpret_cast<uint32_t*>(p.sf) + (((long long)group * (row_pieces / (128 / FP4_QUANT_ROWS)) + (r0 >> 7)) * p.k_blocks + kb) * (WORDS * 128);
+    for (int w = threadIdx.x; w < WORDS * FP4_QUANT_ROWS; w += FP4_QUANT_THREADS) {
+        // neighbouring threads: the words of rows i and i + 32 lie side by side
+        const int t = w / FP4_QUANT_ROWS, i = ((w & 1) << 5) + ((w % FP4_QUANT_ROWS) >> 1), r = r0 + i;
         // rows that are left alone keep their scales; those behind the last one are zero
-        if (p.src == nullptr || r >= p.rows || __ldg(p.src + r) >= 0) out[w] = tile[w];
+        if (p.src == nullptr || r >= p.rows || __ldg(p.src + r) >= 0) out[t * 128 + (r & 31) * 4 + ((r >> 5) & 3)] = tile[t][i];
     }
 }
 

@@ -16,6 +16,18 @@ void with_dtype(int dtype, F f) {
     else f(float{});
 }
 
+// Raises a kernel's dynamic shared memory limit, once per device; `done` belongs to the kernel.
+template <typename K>
+int raise_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    CUDA_TRY(cudaGetDevice(&dev));              // below 64: device_info has been called
+    const uint64_t bit = 1ull << dev;
+    if (done.load(std::memory_order_acquire) & bit) return MOE_OK;
+    CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done.fetch_or(bit, std::memory_order_release);
+    return MOE_OK;
+}
+
 int check_norm(int32_t T, int32_t H, int32_t dtype, int32_t w_dtype) {
     if (T < 0 || H <= 0 || H % 8 || H > NORM_MAX_H)
         return fail(MOE_ERR_INVALID, "T=%d must be non-negative and H=%d a multiple of 8 in [8, %d]", T, H, NORM_MAX_H);
@@ -30,27 +42,75 @@ int check_rows(const char* name, const void* p, int64_t stride, int32_t H) {
     return MOE_OK;
 }
 
-// Threads and 8-column pieces per thread: one piece up to 512 threads, then two or four.
+// Threads and 8-column pieces per thread.  Two pieces: what a row costs every warp (the sum over the block, the wait, its
+// scalars) is shared by more columns than with one -- 16384 x 2048 bf16 forward 44 us against 50, backward 47 against 56 --
+// and four need too many registers (46 and 51 us); they serve rows that 512 threads cannot hold otherwise.
 struct NormShape { int threads, pieces; };
 NormShape norm_shape(int H) {
     const int n8 = H / 8;
     NormShape s;
-    s.pieces = n8 <= NORM_MAX_THREADS ? 1 : (n8 <= 2 * NORM_MAX_THREADS ? 2 : 4);
+    s.pieces = n8 <= 2 * NORM_MAX_THREADS ? 2 : 4;
     s.threads = ((n8 + s.pieces - 1) / s.pieces + 31) / 32 * 32;
     return s;
 }
 
-template <typename T, typename W>
-void launch_norm(const NormParams& p, NormShape s, cudaStream_t st) {
-    if (s.pieces == 1) rms_norm_quant_kernel<T, W, 1><<<p.T, s.threads, 0, st>>>(p);
-    else if (s.pieces == 2) rms_norm_quant_kernel<T, W, 2><<<p.T, s.threads, 0, st>>>(p);
-    else rms_norm_quant_kernel<T, W, 4><<<p.T, s.threads, 0, st>>>(p);
+// Blocks per SM and rows of the ring: as many threads as the registers allow (two blocks of 448 threads forward, one
+// backward), and up to four rows each, which is several times the 45 KB per SM that cover memory's latency.
+struct NormPlan { int per_sm, stages; size_t smem; };
+NormPlan norm_plan(NormShape s, size_t stage_bytes, int threads_per_sm, int most_per_sm) {
+    constexpr size_t room = 200 * 1024;
+    NormPlan n;
+    n.per_sm = threads_per_sm / s.threads;
+    if (n.per_sm > most_per_sm) n.per_sm = most_per_sm;
+    while (n.per_sm > 1 && (size_t)n.per_sm * (2 * stage_bytes + NORM_HEAD_BYTES) > room) --n.per_sm;
+    if (n.per_sm < 1) n.per_sm = 1;
+    n.stages = NORM_MAX_STAGES;
+    while (n.stages > 1 && (size_t)n.per_sm * (n.stages * stage_bytes + NORM_HEAD_BYTES) > room) --n.stages;
+    n.smem = NORM_HEAD_BYTES + n.stages * stage_bytes;
+    return n;
+}
+
+constexpr int NORM_GRAD_THREADS = 768, NORM_GRAD_PER_SM = 12;         // per SM: threads, and blocks at most
+// rows of fp32 that the blocks' shares of dw may take
+int norm_grad_parts(int H) {
+    const int per_sm = NORM_GRAD_THREADS / norm_shape(H).threads;
+    return 160 * (per_sm < 1 ? 1 : (per_sm > NORM_GRAD_PER_SM ? NORM_GRAD_PER_SM : per_sm));
+}
+
+template <typename T, typename W, int CH>
+int launch_norm_ch(NormParams p, NormShape s, DeviceInfo* di, cudaStream_t st) {
+    const NormPlan n = norm_plan(s, (size_t)p.H * sizeof(T) * (p.residual ? 2 : 1), 1024, 24);
+    p.stages = n.stages; p.status = di->status;
+    const int grid = p.T < n.per_sm * di->num_sms ? p.T : n.per_sm * di->num_sms;
+    static std::atomic<uint64_t> done{0};
+    if (int rc = raise_smem(rms_norm_quant_kernel<T, W, CH>, 227 * 1024, done)) return rc;
+    rms_norm_quant_kernel<T, W, CH><<<grid, s.threads, n.smem, st>>>(p);
+    CUDA_TRY(cudaGetLastError());
+    return MOE_OK;
 }
 template <typename T, typename W>
-void launch_norm_grad(const NormGradParams& p, int grid, NormShape s, cudaStream_t st) {
-    if (s.pieces == 1) rms_norm_grad_kernel<T, W, 1><<<grid, s.threads, 0, st>>>(p);
-    else if (s.pieces == 2) rms_norm_grad_kernel<T, W, 2><<<grid, s.threads, 0, st>>>(p);
-    else rms_norm_grad_kernel<T, W, 4><<<grid, s.threads, 0, st>>>(p);
+int launch_norm(const NormParams& p, NormShape s, DeviceInfo* di, cudaStream_t st) {
+    if (s.pieces == 2) return launch_norm_ch<T, W, 2>(p, s, di, st);
+    return launch_norm_ch<T, W, 4>(p, s, di, st);
+}
+template <typename T, typename W, int CH>
+int launch_norm_grad_ch(NormGradParams p, float* dw, NormShape s, DeviceInfo* di, cudaStream_t st) {
+    const NormPlan n = norm_plan(s, (size_t)p.H * sizeof(T) * (p.dh ? 3 : 2), NORM_GRAD_THREADS, NORM_GRAD_PER_SM);
+    p.stages = n.stages; p.status = di->status;
+    int grid = n.per_sm * di->num_sms;
+    if (grid > norm_grad_parts(p.H)) grid = norm_grad_parts(p.H);
+    if (grid > p.T) grid = p.T;
+    static std::atomic<uint64_t> done{0};
+    if (int rc = raise_smem(rms_norm_grad_kernel<T, W, CH>, 227 * 1024, done)) return rc;
+    rms_norm_grad_kernel<T, W, CH><<<grid, s.threads, n.smem, st>>>(p);
+    CUDA_TRY(cudaGetLastError());
+    CUDA_TRY(launch_pdl(rms_norm_dw_kernel, dim3((p.H + 31) / 32), dim3(1024), 0, st, (const float*)p.partial, dw, grid, p.H));
+    return MOE_OK;
+}
+template <typename T, typename W>
+int launch_norm_grad(const NormGradParams& p, float* dw, NormShape s, DeviceInfo* di, cudaStream_t st) {
+    if (s.pieces == 2) return launch_norm_grad_ch<T, W, 2>(p, dw, s, di, st);
+    return launch_norm_grad_ch<T, W, 4>(p, dw, s, di, st);
 }
 
 int check_route(int32_t T, int32_t E, int32_t top_k, int32_t dtype, int32_t score, int64_t stride) {
@@ -123,7 +183,8 @@ int launch_fp4_pair(const GGFp4Params& p, long long rows_total, DeviceInfo* di, 
     const long long blocks = MASKED ? (long long)p.G * ((p.M + 255) / 256) : (p.M + 255) / 256;
     const long long tiles = blocks * sp.num_n_blocks;
     const int pairs = (int)(tiles < di->max_pairs ? tiles : di->max_pairs);
-    CUDA_TRY(cudaFuncSetAttribute((gg_fp4_pair_kernel<NV, MASKED, TN>), cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES));
+    static std::atomic<uint64_t> done{0};
+    if ((rc = raise_smem(gg_fp4_pair_kernel<NV, MASKED, TN>, C::SMEM_BYTES, done)) != MOE_OK) return rc;
     gg_fp4_pair_kernel<NV, MASKED, TN><<<2 * pairs, f4::THREADS, C::SMEM_BYTES, st>>>(ta, tb, tsa, tsb, p, sp, di->status);
     CUDA_TRY(cudaGetLastError());
     return MOE_OK;
@@ -182,7 +243,9 @@ int moe_rms_norm_quant(const moe_norm_args* a, void* stream) {
         return fail(MOE_ERR_INVALID, "weight, q, scales, rstd (and h, with a residual) must be non-NULL");
     if (!aligned16(a->weight) || !aligned16(a->q) || !aligned16(a->h) || !aligned16(a->y))
         return fail(MOE_ERR_INVALID, "weight, q, h and y must be 16-byte aligned");
-    NormParams p;
+    DeviceInfo* di = nullptr;
+    if ((rc = device_info(&di)) != MOE_OK) return rc;
+    NormParams p = {};
     p.x = a->x; p.x_stride = a->x_stride; p.residual = a->residual; p.res_stride = a->residual_stride;
     p.weight = a->weight; p.q = static_cast<uint8_t*>(a->q); p.scales = a->scales; p.ss_row = a->ss_row; p.ss_blk = a->ss_blk;
     p.h = a->h; p.y = a->y; p.rstd = a->rstd; p.T = a->T; p.H = a->H; p.eps = a->eps; p.pow2 = a->pow2 ? 1 : 0;
@@ -190,16 +253,15 @@ int moe_rms_norm_quant(const moe_norm_args* a, void* stream) {
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     with_dtype(a->dtype, [&](auto t) {
         using T = decltype(t);
-        if (a->w_dtype == a->dtype) launch_norm<T, T>(p, s, st);
-        else launch_norm<T, float>(p, s, st);
+        rc = a->w_dtype == a->dtype ? launch_norm<T, T>(p, s, di, st) : launch_norm<T, float>(p, s, di, st);
     });
-    CUDA_TRY(cudaGetLastError());
-    return MOE_OK;
+    return rc;
 }
 
 size_t moe_rms_norm_backward_workspace_bytes(int32_t T, int32_t H) {
-    if (T < 0 || H <= 0) return 0;
-    return align256((size_t)(T < NORM_GRAD_MAX_PARTS ? (T > 0 ? T : 1) : NORM_GRAD_MAX_PARTS) * (size_t)H * 4);
+    if (T < 0 || H <= 0 || H > NORM_MAX_H) return 0;
+    const int parts = norm_grad_parts(H);
+    return align256((size_t)(T < parts ? (T > 0 ? T : 1) : parts) * (size_t)H * 4);
 }
 
 int moe_rms_norm_backward(const moe_norm_grad_args* a, void* stream) {
@@ -221,22 +283,15 @@ int moe_rms_norm_backward(const moe_norm_grad_args* a, void* stream) {
         return fail(MOE_ERR_INVALID, "workspace too small or not 16-byte aligned (moe_rms_norm_backward_workspace_bytes)");
     DeviceInfo* di = nullptr;
     if ((rc = device_info(&di)) != MOE_OK) return rc;
-    NormGradParams p;
+    NormGradParams p = {};
     p.dy = a->dy; p.dy_stride = a->dy_stride; p.h = a->h; p.h_stride = a->h_stride; p.weight = a->weight; p.rstd = a->rstd;
     p.dh = a->dh; p.dh_stride = a->dh_stride; p.dx = a->dx; p.partial = static_cast<float*>(a->workspace); p.T = a->T; p.H = a->H;
     const NormShape s = norm_shape(a->H);
-    int grid = 2 * di->num_sms;
-    if (grid > NORM_GRAD_MAX_PARTS) grid = NORM_GRAD_MAX_PARTS;
-    if (grid > a->T) grid = a->T;
     with_dtype(a->dtype, [&](auto t) {
         using T = decltype(t);
-        if (a->w_dtype == a->dtype) launch_norm_grad<T, T>(p, grid, s, st);
-        else launch_norm_grad<T, float>(p, grid, s, st);
+        rc = a->w_dtype == a->dtype ? launch_norm_grad<T, T>(p, a->dw, s, di, st) : launch_norm_grad<T, float>(p, a->dw, s, di, st);
     });
-    CUDA_TRY(cudaGetLastError());
-    rms_norm_dw_kernel<<<(a->H + 31) / 32, 1024, 0, st>>>(p.partial, a->dw, grid, a->H);
-    CUDA_TRY(cudaGetLastError());
-    return MOE_OK;
+    return rc;
 }
 
 int moe_route(const moe_route_args* a, void* stream) {
@@ -294,7 +349,7 @@ int moe_quant_fp4(const moe_fp4_quant_args* a, void* stream) {
     p.x = a->x; p.x_stride = a->x_stride; p.factor = a->factor; p.factor_stride = a->factor_stride; p.src = a->src_pair; p.top_k = a->top_k;
     p.q = static_cast<uint8_t*>(a->q); p.sf = static_cast<uint8_t*>(a->scales); p.rows = a->rows; p.K = a->K;
     p.gate_first = a->gate_first ? 1 : 0; p.src_rows = a->src_rows; p.k_blocks = (a->K + 255) / 256;
-    const long long blocks = (long long)((a->rows + 127) / 128) * p.k_blocks;
+    const long long blocks = (long long)((a->rows + 127) / 128) * (128 / FP4_QUANT_ROWS) * p.k_blocks;
     if (blocks > 0x7FFFFFFFll) return fail(MOE_ERR_INVALID, "rows x K exceeds what one call covers");
     const dim3 grid((unsigned)blocks, a->groups, 1);
     with_dtype(a->dtype, [&](auto t) {

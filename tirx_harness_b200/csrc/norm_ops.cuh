@@ -3,9 +3,11 @@
 // forward, one row:   h = round(x + residual)              (in the inputs' type: the stream the next layer reads)
 //                     rstd = (sum h^2 / H + eps) ^ -1/2     y = h * rstd * w
 //                     per 128 columns: s = max(amax|y|, 1e-8) / 448 (or that, rounded up to a power of two), q = e4m3(y / s)
-// gradient, one row:  g = dy * w,  dx = rstd * g - h * rstd^3 / H * sum(g h)  (+ dh),  dw = sum over rows of dy * h * rstd
+// gradient, one row:  g = dy * w,  dx = rstd * (g - n * mean(g n)) (+ dh),  n = h * rstd;  dw = sum over rows of dy * n
 //
-// Both are bound by memory: a row is read once, held in registers between the sum and the output, and written once.
+// Both are bound by memory: a row is read once, held in registers between the sum and the output, and written once.  What
+// keeps memory busy is the number of rows under way, not the number of threads: blocks stay on their SM and walk the rows
+// with a stride, and bulk copies bring the next rows into a ring in shared memory while the current one is worked on.
 // Every sum is kept in fp32.
 #pragma once
 
@@ -25,94 +27,133 @@ struct NormParams {
     int T, H;
     float eps;
     int pow2;
+    int stages;                // rows of the ring
+    int* status;
 };
 
-// Sum over the block; every thread gets it.  `buf` holds 33 floats.
+constexpr int NORM_MAX_THREADS = 512;
+constexpr int NORM_MAX_H = 512 * 4 * 8;        // four pieces of 8 columns per thread
+constexpr int NORM_MAX_STAGES = 4;
+constexpr int NORM_HEAD_BYTES = 512;           // shared memory in front of the ring: barriers, sums, flags
+
+// The ring of rows: `streams` inputs of `row_bytes` each per stage.  Thread 0 issues, everybody waits.
+struct RowRing {
+    uint64_t* full;
+    uint8_t* data;
+    volatile int* abort_flag;
+    int* status;
+    int stages, row_bytes, streams;
+    int stage = 0;
+    uint32_t phase = 0;
+
+    __device__ __forceinline__ RowRing(uint8_t* smem, int stages_, int row_bytes_, int streams_, int* status_)
+        : full(reinterpret_cast<uint64_t*>(smem)), data(smem + NORM_HEAD_BYTES),
+          abort_flag(reinterpret_cast<volatile int*>(smem + 64)), status(status_), stages(stages_), row_bytes(row_bytes_), streams(streams_) {
+        if (threadIdx.x == 0) {
+            for (int s = 0; s < stages; ++s) mbar_init(smem_u32(full + s), 1);
+            *abort_flag = 0;
+            fence_mbar_init();
+        }
+        __syncthreads();
+    }
+    __device__ __forceinline__ uint8_t* at(int s, int stream) const { return data + (s * streams + stream) * row_bytes; }
+    __device__ __forceinline__ void expect(int s) const { mbar_arrive_expect_tx(smem_u32(full + s), row_bytes * streams); }
+    __device__ __forceinline__ void load(int s, int stream, const void* src) const {
+        bulk_load(smem_u32(at(s, stream)), src, row_bytes, smem_u32(full + s));
+    }
+    // A wait that runs out sets the status word; the row is then made of whatever the stage holds.
+    __device__ __forceinline__ void wait() const { mbar_wait_warp(smem_u32(full + stage), phase, abort_flag, status, STATUS_TIMEOUT_SMEM_FULL); }
+    __device__ __forceinline__ void next() { if (++stage == stages) { stage = 0; phase ^= 1; } }
+};
+
+// Sum over the block; every thread gets it.  One barrier: two buffers used in turn keep the next sum's writes from this one's reads.
 __device__ __forceinline__ float block_sum(float v, float* buf) {
     v = warp_sum(v);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     if (lane == 0) buf[warp] = v;
     __syncthreads();
-    // every warp adds the partial sums up for itself, in the same order: one barrier instead of two
-    float s = lane < warps ? buf[lane] : 0.0f;
-    return warp_sum(s);
+    return warp_sum(lane < warps ? buf[lane] : 0.0f);          // every warp for itself, in the same order
 }
 
-constexpr int NORM_MAX_THREADS = 512;
-constexpr int NORM_MAX_H = 512 * 4 * 8;        // four pieces of 8 columns per thread
-constexpr int NORM_GRAD_MAX_PARTS = 512;
-
-// One block per row; thread t holds the 8-column pieces t, t + blockDim, ... (CH of them).  A 128-column block is 16
-// neighbouring threads of one piece, so its largest value takes four shuffles.
+// Thread t holds the 8-column pieces t, t + blockDim, ... (CH of them).  A 128-column block is 16 neighbouring threads of
+// one piece, so its largest value takes four shuffles.
 template <typename T, typename W, int CH>
 __global__ void __launch_bounds__(NORM_MAX_THREADS) rms_norm_quant_kernel(const NormParams p) {
-    __shared__ float buf[32];
-    const int row = blockIdx.x, n8 = p.H >> 3;
-    const T* xr = static_cast<const T*>(p.x) + row * p.x_stride;
-    const T* rr = p.residual ? static_cast<const T*>(p.residual) + row * p.res_stride : nullptr;
-    Pack8<T> xv[CH], rv[CH];
-    Pack8<W> wv[CH];
+    extern __shared__ __align__(128) uint8_t smem[];
+    float* sums = reinterpret_cast<float*>(smem + 128);
+    const int n8 = p.H >> 3, step = gridDim.x;
+    const bool res = p.residual != nullptr;
+    RowRing ring(smem, p.stages, p.H * (int)sizeof(T), res ? 2 : 1, p.status);
+    auto fetch = [&](int s, int row) {
+        ring.expect(s);
+        ring.load(s, 0, static_cast<const T*>(p.x) + row * p.x_stride);
+        if (res) ring.load(s, 1, static_cast<const T*>(p.residual) + row * p.res_stride);
+    };
+    if (threadIdx.x == 0)
+        for (int s = 0; s < p.stages && (long long)blockIdx.x + (long long)s * step < p.T; ++s) fetch(s, blockIdx.x + s * step);
+    Raw8<W> wv[CH];
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int i = c * blockDim.x + threadIdx.x;
-        if (i < n8) {
-            xv[c] = load8_once(xr + i * 8);
-            if (rr) rv[c] = load8_once(rr + i * 8);
-            wv[c] = load8(static_cast<const W*>(p.weight) + i * 8);
-        }
+        if (i < n8) wv[c] = load8(static_cast<const W*>(p.weight) + i * 8);
     }
-    float sq = 0.0f;
+    int flip = 0;
+    for (int row = blockIdx.x; row < p.T; flip ^= 32) {
+        ring.wait();
+        f32x2 h[CH][4];
+        f32x2 sq = 0;
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-        const int i = c * blockDim.x + threadIdx.x;
-        if (i < n8) {
-            if (rr) {
+        for (int c = 0; c < CH; ++c) {
+            const int i = c * blockDim.x + threadIdx.x;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) xv[c].v[j] = from_f32<T>(to_f32(xv[c].v[j]) + to_f32(rv[c].v[j]));
-                store8(static_cast<T*>(p.h) + (long long)row * p.H + i * 8, xv[c]);
+            for (int j = 0; j < 4; ++j) h[c][j] = 0;
+            if (i < n8) {
+                unpack8(lds8(reinterpret_cast<const T*>(ring.at(ring.stage, 0)) + i * 8), h[c]);
+                if (res) {
+                    f32x2 r[4];
+                    unpack8(lds8(reinterpret_cast<const T*>(ring.at(ring.stage, 1)) + i * 8), r);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) h[c][j] = add2(h[c][j], r[j]);
+                    const Raw8<T> o = pack8<T>(h[c]);
+                    store8(static_cast<T*>(p.h) + (long long)row * p.H + i * 8, o);
+                    unpack8(o, h[c]);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sq = fma2(h[c][j], h[c][j], sq);
+            }
+        }
+        const float total = block_sum(lo2(sq) + hi2(sq), sums + flip);
+        // the stage has been read by every thread: it can take the row after those under way
+        const long long ahead = (long long)row + (long long)p.stages * step;
+        if (threadIdx.x == 0 && ahead < p.T) fetch(ring.stage, (int)ahead);
+        ring.next();
+        const float rstd = __frsqrt_rn(__fdiv_rn(total, (float)p.H) + p.eps);
+        if (threadIdx.x == 0) p.rstd[row] = rstd;
+        const f32x2 rstd2 = both(rstd);
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int i = c * blockDim.x + threadIdx.x;
+            f32x2 w[4];
+            unpack8(wv[c], w);
+            float amax = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                h[c][j] = i < n8 ? mul2(mul2(h[c][j], rstd2), w[j]) : 0;
+                amax = amax_nan(amax_nan(amax, lo2(h[c][j])), hi2(h[c][j]));
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) { const float f = to_f32(xv[c].v[j]); sq = fmaf(f, f, sq); }
+            for (int o = 8; o > 0; o >>= 1) amax = amax_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+            if (i < n8) {
+                float s = __fdiv_rn(amax < 1.0e-8f ? 1.0e-8f : amax, 448.0f);          // a NaN stays one
+                if (p.pow2 && s < INFINITY) s = __uint_as_float((__float_as_uint(s) + 0x7FFFFFu) & 0xFF800000u);     // up to the next power of two
+                if ((i & 15) == 0) p.scales[row * p.ss_row + (i >> 4) * p.ss_blk] = s;
+                if (p.y) store8(static_cast<T*>(p.y) + (long long)row * p.H + i * 8, pack8<T>(h[c]));
+                div8(h[c], s);
+                *reinterpret_cast<uint2*>(p.q + (long long)row * p.H + i * 8) = pack8_e4m3(h[c]);
+            }
         }
-    }
-    const float rstd = __frsqrt_rn(__fdiv_rn(block_sum(sq, buf), (float)p.H) + p.eps);
-    if (threadIdx.x == 0) p.rstd[row] = rstd;
-#pragma unroll
-    for (int c = 0; c < CH; ++c) {
-        const int i = c * blockDim.x + threadIdx.x;
-        float y[8];
-        uint32_t amax = 0;                  // largest magnitude as bits: infinities and NaN order above every number
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            y[j] = i < n8 ? __fmul_rn(__fmul_rn(to_f32(xv[c].v[j]), rstd), to_f32(wv[c].v[j])) : 0.0f;
-            amax = max(amax, __float_as_uint(y[j]) & 0x7FFFFFFFu);
-        }
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        if (i >= n8) continue;              // no shuffle below
-        const float a = __uint_as_float(amax);
-        float s = __fdiv_rn(a < 1.0e-8f ? 1.0e-8f : a, 448.0f);          // a NaN stays one
-        if (p.pow2 && s < INFINITY) {
-            const uint32_t b = __float_as_uint(s);
-            s = __uint_as_float((b + 0x7FFFFFu) & 0xFF800000u);          // up to the next power of two
-        }
-        uint2 q;
-        if (div_ok(s)) {
-            const float r = __frcp_rn(s);
-            q.x = pack4_e4m3(div_by(y[0], s, r), div_by(y[1], s, r), div_by(y[2], s, r), div_by(y[3], s, r));
-            q.y = pack4_e4m3(div_by(y[4], s, r), div_by(y[5], s, r), div_by(y[6], s, r), div_by(y[7], s, r));
-        } else {
-            q.x = pack4_e4m3(__fdiv_rn(y[0], s), __fdiv_rn(y[1], s), __fdiv_rn(y[2], s), __fdiv_rn(y[3], s));
-            q.y = pack4_e4m3(__fdiv_rn(y[4], s), __fdiv_rn(y[5], s), __fdiv_rn(y[6], s), __fdiv_rn(y[7], s));
-        }
-        *reinterpret_cast<uint2*>(p.q + (long long)row * p.H + i * 8) = q;
-        if ((i & 15) == 0) p.scales[row * p.ss_row + (i >> 4) * p.ss_blk] = s;
-        if (p.y) {
-            Pack8<T> o;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) o.v[j] = from_f32<T>(y[j]);
-            store8(static_cast<T*>(p.y) + (long long)row * p.H + i * 8, o);
-        }
+        if (p.T - row <= step) break;          // row + step could pass 2^31
+        row += step;
     }
 }
 
@@ -125,87 +166,105 @@ struct NormGradParams {
     void* dx;
     float* partial;                           // [gridDim.x, H]: each block's share of dw
     int T, H;
+    int stages;
+    int* status;
 };
 
-// Blocks walk the rows with a stride; a thread keeps its columns' share of dw in registers all the while, so dw costs
-// one row of fp32 per block instead of a second pass over dy and h.
+// A thread keeps its columns' share of dw in registers over all rows of its block, so dw costs one row of fp32 per block
+// instead of a second pass over dy and h.
 template <typename T, typename W, int CH>
 __global__ void __launch_bounds__(NORM_MAX_THREADS) rms_norm_grad_kernel(const NormGradParams p) {
-    __shared__ float buf[2][32];
-    const int n8 = p.H >> 3;
-    float dw[CH][8];
-    Pack8<W> wv[CH];
+    extern __shared__ __align__(128) uint8_t smem[];
+    float* sums = reinterpret_cast<float*>(smem + 128);
+    const int n8 = p.H >> 3, step = gridDim.x;
+    const bool past = p.dh != nullptr;
+    RowRing ring(smem, p.stages, p.H * (int)sizeof(T), past ? 3 : 2, p.status);
+    auto fetch = [&](int s, int row) {
+        ring.expect(s);
+        ring.load(s, 0, static_cast<const T*>(p.dy) + row * p.dy_stride);
+        ring.load(s, 1, static_cast<const T*>(p.h) + row * p.h_stride);
+        if (past) ring.load(s, 2, static_cast<const T*>(p.dh) + row * p.dh_stride);
+    };
+    if (threadIdx.x == 0)
+        for (int s = 0; s < p.stages && (long long)blockIdx.x + (long long)s * step < p.T; ++s) fetch(s, blockIdx.x + s * step);
+    f32x2 dw[CH][4];
+    Raw8<W> wv[CH];
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int i = c * blockDim.x + threadIdx.x;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) dw[c][j] = 0.0f;
+        for (int j = 0; j < 4; ++j) dw[c][j] = 0;
         if (i < n8) wv[c] = load8(static_cast<const W*>(p.weight) + i * 8);
     }
-    int flip = 0;                             // two buffers: one barrier per row is enough
-    for (int row = blockIdx.x; row < p.T; row += gridDim.x, flip ^= 1) {
-        const T* dyr = static_cast<const T*>(p.dy) + row * p.dy_stride;
-        const T* hr = static_cast<const T*>(p.h) + row * p.h_stride;
-        const T* dhr = p.dh ? static_cast<const T*>(p.dh) + row * p.dh_stride : nullptr;
-        Pack8<T> dyv[CH], hv[CH], dv[CH];
-#pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            const int i = c * blockDim.x + threadIdx.x;
-            if (i < n8) {
-                dyv[c] = load8_once(dyr + i * 8);
-                hv[c] = load8_once(hr + i * 8);
-                if (dhr) dv[c] = load8_once(dhr + i * 8);
-            }
-        }
+    int flip = 0;
+    for (int row = blockIdx.x; row < p.T; flip ^= 32) {
         const float rstd = __ldg(p.rstd + row);
-        float dot = 0.0f;
+        const f32x2 rstd2 = both(rstd);
+        ring.wait();
+        Raw8<T> dyv[CH], hv[CH], dhv[CH];
+        f32x2 dot = 0;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int i = c * blockDim.x + threadIdx.x;
             if (i < n8) {
+                dyv[c] = lds8(reinterpret_cast<const T*>(ring.at(ring.stage, 0)) + i * 8);
+                hv[c] = lds8(reinterpret_cast<const T*>(ring.at(ring.stage, 1)) + i * 8);
+                if (past) dhv[c] = lds8(reinterpret_cast<const T*>(ring.at(ring.stage, 2)) + i * 8);
+                f32x2 d[4], n[4], w[4];
+                unpack8(dyv[c], d);
+                unpack8(hv[c], n);
+                unpack8(wv[c], w);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float d = to_f32(dyv[c].v[j]), n = to_f32(hv[c].v[j]) * rstd;
-                    dw[c][j] = fmaf(d, n, dw[c][j]);
-                    dot = fmaf(d * to_f32(wv[c].v[j]), n, dot);
+                for (int j = 0; j < 4; ++j) {
+                    n[j] = mul2(n[j], rstd2);
+                    dw[c][j] = fma2(d[j], n[j], dw[c][j]);
+                    dot = fma2(mul2(d[j], w[j]), n[j], dot);
                 }
             }
         }
-        const float mean = __fdiv_rn(block_sum(dot, buf[flip]), (float)p.H);
+        const float mean = __fdiv_rn(block_sum(lo2(dot) + hi2(dot), sums + flip), (float)p.H);
+        const long long ahead = (long long)row + (long long)p.stages * step;
+        if (threadIdx.x == 0 && ahead < p.T) fetch(ring.stage, (int)ahead);
+        ring.next();
+        const f32x2 minus_mean = both(-mean);
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int i = c * blockDim.x + threadIdx.x;
             if (i < n8) {
-                Pack8<T> o;
+                f32x2 d[4], n[4], w[4];
+                unpack8(dyv[c], d);
+                unpack8(hv[c], n);
+                unpack8(wv[c], w);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float g = to_f32(dyv[c].v[j]) * to_f32(wv[c].v[j]), n = to_f32(hv[c].v[j]) * rstd;
-                    float v = rstd * fmaf(-n, mean, g);
-                    if (dhr) v += to_f32(dv[c].v[j]);
-                    o.v[j] = from_f32<T>(v);
+                for (int j = 0; j < 4; ++j) d[j] = mul2(rstd2, fma2(mul2(n[j], rstd2), minus_mean, mul2(d[j], w[j])));
+                if (past) {
+                    unpack8(dhv[c], n);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) d[j] = add2(d[j], n[j]);
                 }
-                store8(static_cast<T*>(p.dx) + (long long)row * p.H + i * 8, o);
+                store8(static_cast<T*>(p.dx) + (long long)row * p.H + i * 8, pack8<T>(d));
             }
         }
+        if (p.T - row <= step) break;
+        row += step;
     }
+    pdl_launch_dependents();                   // the kernel that adds the shares up may be scheduled; it waits for this one's end
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int i = c * blockDim.x + threadIdx.x;
-        if (i < n8) {
-            float4* dst = reinterpret_cast<float4*>(p.partial + (long long)blockIdx.x * p.H + i * 8);
-            dst[0] = make_float4(dw[c][0], dw[c][1], dw[c][2], dw[c][3]);
-            dst[1] = make_float4(dw[c][4], dw[c][5], dw[c][6], dw[c][7]);
-        }
+        if (i < n8) store8(p.partial + (long long)blockIdx.x * p.H + i * 8, pack8<float>(dw[c]));
     }
 }
 
 // dw[c] = sum of the blocks' shares, always in the same order.  Block: 32 columns x 32 strands of blocks.
-__global__ void __launch_bounds__(1024) rms_norm_dw_kernel(const float* __restrict__ partial, float* __restrict__ dw, int parts, int H) {
+__global__ void __launch_bounds__(1024) rms_norm_dw_kernel(const float* partial, float* __restrict__ dw, int parts, int H) {
     __shared__ float t[32][33];
     const int c = blockIdx.x * 32 + (threadIdx.x & 31), strand = threadIdx.x >> 5;
     float s = 0.0f;
+    pdl_wait();
     if (c < H)
-        for (int i = strand; i < parts; i += 32) s += __ldg(partial + (long long)i * H + c);
+#pragma unroll 8
+        for (int i = strand; i < parts; i += 32) s += partial[(long long)i * H + c];
     t[strand][threadIdx.x & 31] = s;
     __syncthreads();
     s = warp_sum(t[threadIdx.x & 31][strand]);
