@@ -127,6 +127,9 @@ bool route_vec(const void* p, int64_t stride, int32_t E, int32_t dtype) {
     return aligned16(p) && stride % n == 0 && E % n == 0;
 }
 
+// consecutive experts that a lane holds
+int route_per_lane(int E) { return E <= 128 ? 4 : (E <= 256 ? 8 : (E <= 512 ? 16 : 32)); }
+
 template <typename T>
 void launch_route(const RouteParams& p, size_t smem, cudaStream_t st) {
     const int grid = (p.T + RT_WARPS - 1) / RT_WARPS, block = RT_WARPS * 32;
@@ -311,7 +314,11 @@ int moe_route(const moe_route_args* a, void* stream) {
     p.ids = a->ids; p.weights = a->weights; p.T = a->T; p.E = a->E; p.top_k = a->top_k; p.n_group = a->n_group;
     p.topk_group = a->topk_group; p.sigmoid = a->score == MOE_SCORE_SIGMOID; p.top2 = a->group_score == MOE_GROUP_TOP2;
     p.renorm = a->renormalize ? 1 : 0; p.vec = route_vec(a->logits, a->stride, a->E, a->dtype); p.scale = a->scale;
-    const size_t smem = a->bias || a->n_group > 1 ? (size_t)RT_WARPS * (a->E + RT_MAX_GROUPS) * 8 : 0;
+    p.bias_vec = route_vec(a->bias, 0, a->E, a->bias_dtype);
+    p.gs = a->E / a->n_group;
+    const int per = route_per_lane(a->E), lanes = p.gs / per;
+    p.group_shift = lanes * per == p.gs && lanes > 0 && (lanes & (lanes - 1)) == 0 ? __builtin_ctz(lanes) : -1;
+    const size_t smem = a->bias || a->n_group > 1 ? (size_t)RT_WARPS * a->E * 8 : 0;
     with_dtype(a->dtype, [&](auto t) { launch_route<decltype(t)>(p, smem, static_cast<cudaStream_t>(stream)); });
     CUDA_TRY(cudaGetLastError());
     return MOE_OK;

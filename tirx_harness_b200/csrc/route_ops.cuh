@@ -12,8 +12,13 @@
 // left, the id is -1 and the weight 0.
 //
 // Which experts are chosen follows the exact order of the keys, ties to the lowest index.  Without a bias that order is
-// the logits' own.  With one, or between groups, the fp32 keys decide only where they are further apart than their error;
-// a token in which two compared keys are closer (a few in a thousand) is chosen again from keys in 64 bits.
+// the logits' own.  With one, or between groups, the fp32 keys decide only where they are further apart than their error
+// (rt_margin); where they are not (a few tokens in a thousand) keys in 64 bits do.
+//
+// Bound by the instructions of the choice, not by memory.  The choice has no round per expert: the best key of each lane is
+// sorted across the warp; the top_k-th of them is a bound that top_k keys at least reach; the few keys that do (about a
+// dozen) are collected, one to a lane, and each counts how many are before it.  16384 x 256 with bias and groups, top 8:
+// 51 us with a reduction over the warp per chosen expert, 20 us like this.
 #pragma once
 
 #include "num_common.cuh"
@@ -30,7 +35,9 @@ struct RouteParams {
     int* ids;
     float* weights;
     int T, E, top_k, n_group, topk_group;
-    int sigmoid, top2, renorm, vec;
+    int sigmoid, top2, renorm, vec, bias_vec;
+    int gs;                             // experts per group
+    int group_shift;                    // a group is 2^group_shift whole lanes; -1: lanes and groups do not match
     float scale;
 };
 
@@ -41,17 +48,32 @@ __device__ __forceinline__ float rt_bias(const RouteParams& p, int e) {
 // larger key = larger number; 0 is below every key
 __device__ __forceinline__ uint32_t rt_order(float f) {
     const uint32_t b = __float_as_uint(f);
-    return (b & 0x80000000u) ? ~b : b | 0x80000000u;
+    return b ^ (((int32_t)b >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float rt_unorder(uint32_t o) {
-    return __uint_as_float((o & 0x80000000u) ? o & 0x7FFFFFFFu : ~o);
+    return __uint_as_float(o ^ (((int32_t)~o >> 31) | 0x80000000u));
 }
-// What two keys of this size may be off together: exp, the division and the additions leave each score (at most 1)
-// within 1e-6, the bias adds half a step of the key.
-__device__ __forceinline__ bool rt_close(float a, float b) { return fabsf(a - b) <= 4e-6f * fmaxf(1.0f, fabsf(a)); }
+// How far apart two fp32 keys must be for their order to be the exact one.  A score is off by less than 3e-7: sigmoid
+// p (1 - p) times the relative error of exp2 (2^-22, and |l| 2^-24 from its argument, where |l| p (1 - p) < 0.28), the
+// reciprocal 2^-23 and the addition 2^-24; softmax the like.  A bias adds half a step of the key.  The sum of a group's two
+// best doubles both.
+__device__ __forceinline__ float rt_margin(float key, bool pair) { return (pair ? 2e-6f : 1e-6f) * fmaxf(1.0f, fabsf(key)); }
+constexpr float RT_BIG = 3.402823466e38f;           // +infinity counts as the largest number
 
-// The E logits of a token in the warp's registers: lane l holds experts l * PER ... l * PER + PER - 1; -infinity where
-// there is none.  vec: whole 16-byte pieces (E, the row distance and the base allow it).
+__device__ __forceinline__ float rt_ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float rt_exp(float x) { return rt_ex2(x * 1.4426950408889634f); }
+__device__ __forceinline__ float rt_sigmoid(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + rt_exp(-x)));
+    return r;
+}
+
+// PER consecutive values; -infinity behind E and for NaN.  vec: whole 16-byte pieces (E, the row distance and the base
+// allow it).
 template <typename T, int PER>
 __device__ __forceinline__ void rt_load(const T* row, int E, int lane, bool vec, float (&l)[PER]) {
     constexpr int VL = PER < (int)(16 / sizeof(T)) ? PER : (int)(16 / sizeof(T));
@@ -69,81 +91,100 @@ __device__ __forceinline__ void rt_load(const T* row, int E, int lane, bool vec,
         for (int j = 0; j < PER; ++j) l[j] = lane * PER + j < E ? to_f32(row[lane * PER + j]) : -INFINITY;
     }
 #pragma unroll
-    for (int j = 0; j < PER; ++j) if (rt_off(l[j])) l[j] = -INFINITY;
+    for (int j = 0; j < PER; ++j) l[j] = fminf(fmaxf(l[j], -INFINITY), RT_BIG);
 }
 
-// Softmax statistics of the row: largest finite logit and 1 / sum of the exponentials (0 where every expert is off).
+// Softmax statistics of the row: its largest logit and 1 / the sum of the exponentials (0 where every expert is off);
+// e[j]: the exponentials, 0 for an expert that is off.
 template <int PER>
-__device__ __forceinline__ void rt_softmax(float (&l)[PER], float* mx, float* inv) {
-    float m = -INFINITY;
+__device__ __forceinline__ void rt_softmax(const float (&l)[PER], float (&e)[PER], float* mx, float* inv) {
+    float m = l[0];
 #pragma unroll
-    for (int j = 0; j < PER; ++j) { l[j] = fminf(l[j], 3.402823466e38f); m = fmaxf(m, l[j]); }
+    for (int j = 1; j < PER; ++j) m = fmaxf(m, l[j]);
     m = warp_max(m);
+    if (m == -INFINITY) m = 0.0f;
     float s = 0.0f;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) s += l[j] == -INFINITY ? 0.0f : expf(l[j] - m);
+    for (int j = 0; j < PER; ++j) {
+        e[j] = rt_exp(l[j] - m);
+        s += e[j];
+    }
     s = warp_sum(s);
     *mx = m;
     *inv = s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f;
 }
+// the score of one expert that is not off, for its weight
 __device__ __forceinline__ float rt_score(float l, bool sigmoid, float mx, float inv) {
-    if (l == -INFINITY) return 0.0f;
-    return sigmoid ? __fdiv_rn(1.0f, 1.0f + expf(-l)) : expf(fminf(l, 3.402823466e38f) - mx) * inv;
+    return sigmoid ? __fdiv_rn(1.0f, 1.0f + expf(-l)) : expf(fminf(l, RT_BIG) - mx) * inv;
 }
 
-// The choice from 64-bit keys, in shared memory.  -> the id of choice `lane` (-1: none).
+// ---- 64 bits, for the tokens whose fp32 keys are too close.  The whole warp takes part in each.
+// Softmax: the row's largest logit and the sum of the exponentials.
 template <typename T>
-__device__ __noinline__ int rt_choose64(const RouteParams& p, const T* row, double* key, double* gscore, int lane) {
-    const double none = -INFINITY;
-    double m = none;
-    for (int e = lane; e < p.E; e += 32) m = fmax(m, (double)(rt_off(to_f32(row[e])) ? -INFINITY : fminf(to_f32(row[e]), 3.402823466e38f)));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, o));
-    double sum = 0;
+__device__ __forceinline__ void rt_softmax64(const RouteParams& p, const T* row, int lane, double* mx, double* sum) {
+    float m = -INFINITY;
+    for (int e = lane; e < p.E; e += 32) m = fmaxf(m, to_f32(row[e]));
+    m = fminf(warp_max(m), RT_BIG);
+    double s = 0.0;
     for (int e = lane; e < p.E; e += 32) {
-        const float lf = to_f32(row[e]);
-        const double l = fminf(lf, 3.402823466e38f);
-        double k = none;
-        if (!rt_off(lf)) {
-            k = p.sigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - m);
-            sum += k;
-        }
-        key[e] = k;
+        const float l = to_f32(row[e]);
+        if (!rt_off(l)) s += exp((double)fminf(l, RT_BIG) - (double)m);
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    *mx = m;
+    *sum = s;
+}
+__device__ __forceinline__ double rt_key64_of(const RouteParams& p, float l, int e, double mx, double sum) {
+    const double k = p.sigmoid ? 1.0 / (1.0 + exp(-(double)l)) : exp((double)fminf(l, RT_BIG) - mx) / sum;
+    return p.bias ? k + (double)rt_bias(p, e) : k;
+}
+// The key of expert `id` (-1: none).
+template <typename T>
+__device__ __noinline__ double rt_key64(const RouteParams& p, const T* row, int id, int lane) {
+    double mx = 0.0, sum = 1.0;
+    if (!p.sigmoid) rt_softmax64<T>(p, row, lane, &mx, &sum);
+    return id >= 0 ? rt_key64_of(p, to_f32(row[id]), id, mx, sum) : -INFINITY;
+}
+// The keys of all experts, -infinity for one that is off.
+template <typename T>
+__device__ __noinline__ void rt_keys64(const RouteParams& p, const T* row, double* key, int lane) {
+    double mx = 0.0, sum = 1.0;
+    if (!p.sigmoid) rt_softmax64<T>(p, row, lane, &mx, &sum);
     for (int e = lane; e < p.E; e += 32) {
-        double k = key[e];
-        if (k != none) {
-            if (!p.sigmoid) k /= sum;
-            if (p.bias) k += (double)rt_bias(p, e);
-        }
-        key[e] = k;
+        const float l = to_f32(row[e]);
+        const double k = rt_off(l) ? (double)-INFINITY : rt_key64_of(p, l, e, mx, sum);
+        key[e] = k > (double)-INFINITY ? k : (double)-INFINITY;          // a NaN in the bias
     }
     __syncwarp();
-    if (p.n_group > 1) {
-        const int gs = p.E / p.n_group;
-        double a = none, b = none;
-        if (lane < p.n_group)
-            for (int i = 0; i < gs; ++i) {
-                const double k = key[lane * gs + i];
-                if (k > a) { b = a; a = k; } else if (k > b) b = k;
-            }
-        const double g = a == none ? none : (p.top2 && b != none ? a + b : a);
-        if (lane < p.n_group) gscore[lane] = g;
-        __syncwarp();
-        int before = 0;
-        if (lane < p.n_group)
-            for (int i = 0; i < p.n_group; ++i) before += gscore[i] > g || (gscore[i] == g && i < lane);
-        if (lane < p.n_group && before >= p.topk_group)
-            for (int i = 0; i < gs; ++i) key[lane * gs + i] = none;
-        __syncwarp();
+}
+// Whether group `lane` is among the topk_group best.
+template <typename T>
+__device__ __noinline__ bool rt_groups64(const RouteParams& p, const T* row, double* key, int lane) {
+    rt_keys64<T>(p, row, key, lane);
+    double a = -INFINITY, b = -INFINITY;
+    if (lane < p.n_group)
+        for (int i = 0; i < p.gs; ++i) {
+            const double k = key[lane * p.gs + i];
+            b = fmax(b, fmin(a, k));
+            a = fmax(a, k);
+        }
+    const double g = p.top2 && b > (double)-INFINITY ? a + b : a;
+    int before = 0;
+    for (int i = 0; i < p.n_group; ++i) {
+        const double o = __shfl_sync(0xffffffffu, g, i);
+        before += o > g || (o == g && i < lane);
     }
+    __syncwarp();
+    return lane < p.n_group && before < p.topk_group;
+}
+// The choice one expert after the other from keys in shared memory -> the id of choice `lane` (-1: none).
+__device__ __noinline__ int rt_choose64(int E, int top_k, double* key, int lane) {
     int mine = -1;
-    for (int k = 0; k < p.top_k; ++k) {
-        double best = none;
+    for (int k = 0; k < top_k; ++k) {
+        double best = -INFINITY;
         int at = -1;
-        for (int e = lane; e < p.E; e += 32)
+        for (int e = lane; e < E; e += 32)
             if (key[e] > best) { best = key[e]; at = e; }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
@@ -153,97 +194,211 @@ __device__ __noinline__ int rt_choose64(const RouteParams& p, const T* row, doub
         }
         if (at < 0) break;
         if (lane == k) mine = at;
-        if (lane == (at & 31)) key[at] = none;
+        if (lane == (at & 31)) key[at] = -INFINITY;
         __syncwarp();
     }
     return mine;
 }
 
-// One warp per token.
+constexpr uint32_t RT_LEAST = 0x00800000u;          // rt_order of the lowest number; -infinity is one less
+
+// One warp per token; lane l holds experts l * PER ... l * PER + PER - 1.
 template <typename T, int PER>
 __global__ void __launch_bounds__(RT_WARPS * 32) route_kernel(const RouteParams p) {
-    extern __shared__ double rt_smem[];              // per warp: E 64-bit keys and the groups' scores
+    extern __shared__ double rt_smem[];              // per warp: E 64-bit keys (where keys are scores)
+    __shared__ unsigned long long cands[RT_WARPS][2][32];          // key << 32 | ~expert: the larger one comes first
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int t = blockIdx.x * RT_WARPS + warp;
     if (t >= p.T) return;
-    double* key64 = rt_smem + (long long)warp * (p.E + RT_MAX_GROUPS);
-    float* skey = reinterpret_cast<float*>(key64);
+    double* key64 = rt_smem + warp * p.E;
     const T* row = static_cast<const T*>(p.logits) + t * p.stride;
-    float l[PER];
+    float l[PER], k[PER];
     rt_load<T, PER>(row, p.E, lane, p.vec, l);
     float mx = 0.0f, inv = 0.0f;
-    if (!p.sigmoid) rt_softmax(l, &mx, &inv);
-    uint32_t key[PER];
-    const bool need_score = p.bias != nullptr || p.n_group > 1;
-    bool close = false;
+    if (!p.sigmoid) rt_softmax(l, k, &mx, &inv);
+    const bool scored = p.bias != nullptr || p.n_group > 1;
+    if (scored) {
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-        const int e = lane * PER + j;
-        float k = l[j];
-        if (need_score && e < p.E) {
-            k = rt_score(l[j], p.sigmoid, mx, inv);
-            if (p.bias) k += rt_bias(p, e);
-            if (l[j] == -INFINITY || !(k > -INFINITY)) k = -INFINITY;
-            skey[e] = k;
+        for (int j = 0; j < PER; ++j) k[j] = p.sigmoid ? rt_sigmoid(l[j]) : k[j] * inv;
+        if (p.bias) {
+            float b[PER];
+            if (p.bias_bf16) rt_load<__nv_bfloat16, PER>(static_cast<const __nv_bfloat16*>(p.bias), p.E, lane, p.bias_vec, b);
+            else rt_load<float, PER>(static_cast<const float*>(p.bias), p.E, lane, p.bias_vec, b);
+#pragma unroll
+            for (int j = 0; j < PER; ++j) k[j] += b[j];
         }
-        key[j] = k == -INFINITY ? 0u : rt_order(p.bias ? k : l[j]);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) k[j] = l[j] == -INFINITY ? -INFINITY : k[j];
     }
-    if (p.n_group > 1) {
-        __syncwarp();
-        const int gs = p.E / p.n_group;
-        float a = -INFINITY, b = -INFINITY;
-        if (lane < p.n_group)
-            for (int i = 0; i < gs; ++i) {
-                const float k = skey[lane * gs + i];
-                if (k > a) { b = a; a = k; } else if (k > b) b = k;
-            }
-        const float g = p.top2 && b > -INFINITY ? a + b : a;
-        int before = 0;
-        for (int i = 0; i < p.n_group; ++i) {
-            const float o = __shfl_sync(0xffffffffu, g, i);
-            before += o > g || (o == g && i < lane);
-            // keys of two groups so close that their order needs 64 bits (both empty: the order does not matter)
-            close |= lane < p.n_group && i != lane && o > -INFINITY && rt_close(o, g);
-        }
-        const unsigned keep = __ballot_sync(0xffffffffu, lane < p.n_group && before < p.topk_group);
+    uint32_t key[PER];
 #pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const int e = lane * PER + j;
-            if (e < p.E && !((keep >> (e / gs)) & 1u)) key[j] = 0u;
+    for (int j = 0; j < PER; ++j) key[j] = rt_order(p.bias ? k[j] : l[j]);
+    if (p.n_group > 1) {
+        const bool even = p.group_shift >= 0;
+        float a = -INFINITY, b = -INFINITY;            // the two best keys of a lane, then of a group
+        if (even) {
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                b = fmaxf(b, fminf(a, k[j]));
+                a = fmaxf(a, k[j]);
+            }
+            for (int o = 1; o < 1 << p.group_shift; o <<= 1) {
+                const float oa = __shfl_xor_sync(0xffffffffu, a, o), ob = __shfl_xor_sync(0xffffffffu, b, o);
+                b = fmaxf(fminf(a, oa), fmaxf(b, ob));
+                a = fmaxf(a, oa);
+            }
+        } else {
+            float* skey = reinterpret_cast<float*>(key64);
+#pragma unroll
+            for (int j = 0; j < PER; ++j) if (lane * PER + j < p.E) skey[lane * PER + j] = k[j];
+            __syncwarp();
+            if (lane < p.n_group)
+                for (int i = 0; i < p.gs; ++i) {
+                    const float v = skey[lane * p.gs + i];
+                    b = fmaxf(b, fminf(a, v));
+                    a = fmaxf(a, v);
+                }
+            __syncwarp();
+        }
+        const int shift = even ? p.group_shift : 0, g_of = lane >> shift;          // lane g << shift has group g's score
+        const float g = p.top2 && b > -INFINITY ? a + b : a, eps = rt_margin(g, true);
+        int before = 0, near = 0;
+        for (int i = 0; i < p.n_group; ++i) {
+            const float o = __shfl_sync(0xffffffffu, g, i << shift);
+            before += o > g || (o == g && i < g_of);
+            near += fabsf(o - g) <= eps;              // itself, and groups whose order needs 64 bits
+        }
+        bool kept = g_of < p.n_group && before < p.topk_group;
+        const bool real = g_of < p.n_group && g > -INFINITY;
+        unsigned keep = __ballot_sync(0xffffffffu, kept);
+        if (__any_sync(0xffffffffu, real && near > 1)) {           // it matters where one is kept and the other is not
+            bool close = false;
+            for (int i = 0; i < p.n_group; ++i) {
+                const float o = __shfl_sync(0xffffffffu, g, i << shift);
+                close |= real && fabsf(o - g) <= eps && kept != (bool)((keep >> (i << shift)) & 1u);
+            }
+            if (__any_sync(0xffffffffu, close)) {
+                const unsigned groups = __ballot_sync(0xffffffffu, rt_groups64<T>(p, row, key64, lane));
+                kept = (groups >> g_of) & 1u;
+                keep = __ballot_sync(0xffffffffu, kept);
+            }
+        }
+        if (even) {
+#pragma unroll
+            for (int j = 0; j < PER; ++j) key[j] = kept ? key[j] : 0u;
+        } else {
+            int g_at = lane * PER / p.gs, left = (g_at + 1) * p.gs - lane * PER;       // of that group from this expert on
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                if (left == 0) { ++g_at; left = p.gs; }
+                --left;
+                if (!((keep >> (g_at & 31)) & 1u)) key[j] = 0u;
+            }
         }
     }
     int mine = -1;
-    float last = INFINITY;
-    const int rounds = p.bias ? p.top_k + 1 : p.top_k;          // with a bias the best one left out is looked at too
-    for (int k = 0; k < rounds; ++k) {
-        uint32_t best = key[0];
-        int at = 0;
+    // with a bias the best key left out is looked at too
+    const int wanted = p.bias ? p.top_k + 1 : p.top_k;
+    uint32_t bound = key[0];
 #pragma unroll
-        for (int j = 1; j < PER; ++j) if (key[j] > best) { best = key[j]; at = j; }
-        const uint32_t m = __reduce_max_sync(0xffffffffu, best);
-        if (m == 0u) break;
-        const int winner = __ffs(__ballot_sync(0xffffffffu, best == m)) - 1;
-        const int e = __shfl_sync(0xffffffffu, lane * PER + at, winner);
-        if (lane == k && k < p.top_k) mine = e;
-        if (lane == winner) {
+    for (int j = 1; j < PER; ++j) bound = max(bound, key[j]);
 #pragma unroll
-            for (int j = 0; j < PER; ++j) if (j == at) key[j] = 0u;
+    for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (int o = size >> 1; o > 0; o >>= 1) {
+            const uint32_t other = __shfl_xor_sync(0xffffffffu, bound, o);
+            const bool larger = ((lane & o) == 0) == ((lane & size) == 0);
+            bound = larger ? max(bound, other) : min(bound, other);
         }
-        if (p.bias) {
-            const float v = rt_unorder(m);
-            close |= rt_close(v, last);
-            last = v;
-        }
+    bound = __shfl_sync(0xffffffffu, bound, min(wanted, 32) - 1);
+    if (p.bias && bound >= RT_LEAST) {              // whatever 64 bits may put among the chosen is collected too
+        const float v = rt_unorder(bound);
+        bound = rt_order(v - rt_margin(v, false));
     }
-    if (need_score && __any_sync(0xffffffffu, close)) {
+    bound = max(bound, RT_LEAST);
+    int count = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) count += key[j] >= bound;
+    int at = count;                                  // where this lane's candidates begin
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, at, o);
+        if (lane >= o) at += v;
+    }
+    const int total = __shfl_sync(0xffffffffu, at, 31);
+    at -= count;
+    if (total <= 32 && wanted <= 32) {
+        unsigned long long* c = cands[warp][0];
+        unsigned long long* sorted = cands[warp][1];
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+            if (key[j] >= bound) c[at++] = (unsigned long long)key[j] << 32 | (uint32_t)~(lane * PER + j);
         __syncwarp();
-        mine = rt_choose64<T>(p, row, key64, key64 + p.E, lane);
+        const unsigned long long me = lane < total ? c[lane] : 0ull;
+        int rank = 0;
+        for (int i = 0; i < total; ++i) rank += c[i] > me;
+        if (lane < total) sorted[rank] = me;
+        __syncwarp();
+        const unsigned long long s = lane < total ? sorted[lane] : 0ull;
+        mine = lane < total ? (int)~(uint32_t)s : -1;
+        if (p.bias) {
+            const float v = rt_unorder((uint32_t)(s >> 32));
+            const float next = __shfl_down_sync(0xffffffffu, v, 1);
+            if (__any_sync(0xffffffffu, lane < p.top_k && lane + 1 < total && v - next <= rt_margin(v, false))) {
+                const double exact = rt_key64<T>(p, row, mine, lane);
+                rank = 0;
+                for (int i = 0; i < total; ++i) {
+                    const double o = __shfl_sync(0xffffffffu, exact, i);
+                    const int oe = __shfl_sync(0xffffffffu, mine, i);
+                    rank += o > exact || (o == exact && oe < mine);
+                }
+                __syncwarp();
+                if (lane < total) c[rank] = s;
+                __syncwarp();
+                if (lane < total) mine = (int)~(uint32_t)c[lane];
+            }
+        }
+    } else {
+        // many equal keys: one after the other
+        bool close = false;
+        float last = INFINITY;
+        unsigned allowed = 0;                        // of this lane's experts
+#pragma unroll
+        for (int j = 0; j < PER; ++j) allowed |= (unsigned)(key[j] >= RT_LEAST) << j;
+        for (int r = 0; r < wanted; ++r) {
+            uint32_t best = key[0];
+            int a = 0;
+#pragma unroll
+            for (int j = 1; j < PER; ++j) if (key[j] > best) { best = key[j]; a = j; }
+            const uint32_t m = __reduce_max_sync(0xffffffffu, best);
+            if (m < RT_LEAST) break;
+            const int winner = __ffs(__ballot_sync(0xffffffffu, best == m)) - 1;
+            const int e = __shfl_sync(0xffffffffu, lane * PER + a, winner);
+            if (lane == r) mine = e;
+            if (lane == winner) {
+#pragma unroll
+                for (int j = 0; j < PER; ++j) if (j == a) key[j] = 0u;
+            }
+            if (p.bias) {
+                const float v = rt_unorder(m);
+                close |= last - v <= rt_margin(v, false);
+                last = v;
+            }
+        }
+        if (close) {                                 // the same in all lanes
+            rt_keys64<T>(p, row, key64, lane);
+            for (int j = 0; j < PER; ++j)
+                if (lane * PER + j < p.E && !((allowed >> j) & 1u)) key64[lane * PER + j] = -INFINITY;
+            __syncwarp();
+            mine = rt_choose64(p.E, p.top_k, key64, lane);
+        }
     }
+    if (lane >= p.top_k) mine = -1;
     const float s = mine >= 0 ? rt_score(to_f32(row[mine]), p.sigmoid, mx, inv) : 0.0f;
-    const float total = warp_sum(s) + 1e-20f;
+    const float total_s = warp_sum(s) + 1e-20f;
     if (lane < p.top_k) {
         p.ids[(long long)t * p.top_k + lane] = mine;
-        p.weights[(long long)t * p.top_k + lane] = (p.renorm ? __fdiv_rn(s, total) : s) * p.scale;
+        p.weights[(long long)t * p.top_k + lane] = (p.renorm ? __fdiv_rn(s, total_s) : s) * p.scale;
     }
 }
 
@@ -256,62 +411,70 @@ struct RouteGradParams {
     float scale;
 };
 
+// One warp per token.  With c_j = dL/dp_j p_j (softmax) or dL/dp_j p_j (1 - p_j) (sigmoid) of the chosen experts, a row is
+// -p_e * sum(c) (softmax) or 0 everywhere, plus c_j at expert j: the row is written first, then the chosen entries.
+// Bound by memory and its latency.
 template <typename T, int PER>
 __global__ void __launch_bounds__(RT_WARPS * 32) route_grad_kernel(const RouteGradParams p) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int t = blockIdx.x * RT_WARPS + warp;
     if (t >= p.T) return;
     const T* row = static_cast<const T*>(p.logits) + t * p.stride;
-    float l[PER];
-    rt_load<T, PER>(row, p.E, lane, p.vec, l);
-    float mx = 0.0f, inv = 0.0f;
-    if (!p.sigmoid) rt_softmax(l, &mx, &inv);
     int id = -1;
-    float g = 0.0f, s = 0.0f;
+    float g = 0.0f, s = 0.0f, li = -INFINITY;
     if (lane < p.top_k) {
         id = __ldg(p.ids + (long long)t * p.top_k + lane);
-        if (id >= p.E) id = -1;
-        if (id >= 0) {
-            float li = to_f32(row[id]);
-            if (rt_off(li)) id = -1;
-            else {
-                s = rt_score(li, p.sigmoid, mx, inv);
-                g = __ldg(p.grad + (long long)t * p.top_k + lane) * p.scale;
-            }
-        }
+        g = __ldg(p.grad + (long long)t * p.top_k + lane) * p.scale;
     }
-    float dot = warp_sum(g * s);
+    float o[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) o[j] = 0.0f;
+    float mx = 0.0f, inv = 0.0f;
+    if (!p.sigmoid) {
+        float l[PER];
+        rt_load<T, PER>(row, p.E, lane, p.vec, l);
+        if (id >= 0 && id < p.E) li = to_f32(row[id]);
+        rt_softmax(l, o, &mx, &inv);
+    } else if (id >= 0 && id < p.E) li = to_f32(row[id]);
+    if (rt_off(li)) {
+        id = -1;
+        g = 0.0f;
+    } else s = rt_score(li, p.sigmoid, mx, inv);
     if (p.renorm) {
         const float total = warp_sum(s) + 1e-20f;
+        const float dot = warp_sum(g * s);
         g = id >= 0 ? __fdiv_rn(g - __fdiv_rn(dot, total), total) : 0.0f;
-        dot = warp_sum(g * s);
     }
-    float ds[PER];
+    float c = g * s, minus = 0.0f;
+    if (p.sigmoid) c *= 1.0f - s;
+    else {
+        minus = -warp_sum(c);
 #pragma unroll
-    for (int j = 0; j < PER; ++j) ds[j] = 0.0f;
-    for (int k = 0; k < p.top_k; ++k) {            // an expert that a token names twice gets both shares
-        const int at = __shfl_sync(0xffffffffu, id, k) - lane * PER;
-        const float v = __shfl_sync(0xffffffffu, g, k);
-#pragma unroll
-        for (int j = 0; j < PER; ++j) if (j == at) ds[j] += v;
+        for (int j = 0; j < PER; ++j) o[j] *= minus * inv;
     }
     T* out = static_cast<T*>(p.out) + (long long)t * p.E;
-    constexpr int VL = PER < (int)(16 / sizeof(T)) ? PER : (int)(16 / sizeof(T));
+    if (p.vec) {
+        constexpr int VL = PER < (int)(16 / sizeof(T)) ? PER : (int)(16 / sizeof(T));
 #pragma unroll
-    for (int j = 0; j < PER; j += VL) {
-        struct alignas(sizeof(T) * VL) V { T v[VL]; } x;
+        for (int j = 0; j < PER; j += VL) {
+            struct alignas(sizeof(T) * VL) V { T v[VL]; } x;
 #pragma unroll
-        for (int i = 0; i < VL; ++i) {
-            const float sc = rt_score(l[j + i], p.sigmoid, mx, inv);
-            x.v[i] = from_f32<T>(p.sigmoid ? ds[j + i] * sc * (1.0f - sc) : sc * (ds[j + i] - dot));
-        }
-        if (p.vec) {
+            for (int i = 0; i < VL; ++i) x.v[i] = from_f32<T>(o[j + i]);
             if (lane * PER + j < p.E) *reinterpret_cast<V*>(out + lane * PER + j) = x;
-        } else {
-#pragma unroll
-            for (int i = 0; i < VL; ++i) if (lane * PER + j + i < p.E) out[lane * PER + j + i] = x.v[i];
         }
+    } else {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) if (lane * PER + j < p.E) out[lane * PER + j] = from_f32<T>(o[j]);
     }
+    // an expert that a token names twice gets both shares: each of its lanes adds them up in the same order
+    float sum = s * minus;
+    for (int k = 0; k < p.top_k; ++k) {
+        const int oid = __shfl_sync(0xffffffffu, id, k);
+        const float oc = __shfl_sync(0xffffffffu, c, k);
+        sum += oid == id ? oc : 0.0f;
+    }
+    __syncwarp();
+    if (id >= 0) out[id] = from_f32<T>(sum);
 }
 
 }  // namespace b200
