@@ -547,6 +547,11 @@ CONTIGUOUS = [
     ((300, 0, 260, 40), (84, 0, 124, 88), 456, 1152, "nvfp4", "fp32"),
     ((17, 19, 23, 29, 31), (0, 0, 0, 0, 5), 264, 2048, "mxfp4", "bf16"),
     ((1, 1, 1, 1, 1, 1, 1, 1), (0,) * 8, 640, 1024, "nvfp4", "bf16"),
+    # at most 32 and 128 rows: several tiles per block, blocks that share K, K shorter than the blocks that share it
+    ((3, 4) * 4, (0,) * 8, 2560, 512, "mxfp4", "fp32"),
+    ((40, 30, 0, 50), (2, 0, 0, 6), 4096, 768, "nvfp4", "bf16"),
+    ((33,), (0,), 1024, 256, "mxfp4", "fp32"),
+    ((20, 2), (0, 0), 1032, 1280, "nvfp4", "fp32"),
 ]
 
 
@@ -596,6 +601,12 @@ MASKED = [
     ((1, 1, 1, 1, 1, 1, 1, 1), 1, 1024, 2048, "nvfp4", "bf16"),
     ((0, 0), 4, 64, 128, "mxfp4", "bf16"),
     ((300, 256, 257), 300, 512, 1024, "mxfp4", "bf16"),
+    # at most 32 and 128 rows: several tiles per block, no tile at all for most groups, blocks that share K
+    (tuple(i % 9 for i in range(48)), 8, 1096, 512, "nvfp4", "bf16"),
+    (tuple(128 - i for i in range(12)), 128, 2048, 384, "mxfp4", "fp32"),
+    (tuple(5 * (i % 200 == 7) for i in range(1024)), 5, 256, 512, "mxfp4", "bf16"),
+    ((100,), 100, 512, 2048, "nvfp4", "fp32"),
+    ((12, 0, 0, 31), 32, 1000, 128, "mxfp4", "fp32"),
 ]
 
 

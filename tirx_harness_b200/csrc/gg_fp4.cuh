@@ -306,4 +306,298 @@ gg_fp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
     }
 }
 
+// ------------------------------------------------------------------ few rows per group
+// gg_fp4_few_kernel: the weights' rows are the MMA's M (128 per tile), the group's rows its N (at most NT = 32 or 128), so a
+// tile streams 128 rows of B over all of K and multiplies little in vain.  Bound by reading the weights from HBM: two
+// blocks per SM (NT = 32) keep four 16 KB stages each under way.  Two accumulators: a tile is stored while the next one is
+// multiplied.  Blocks come in clusters of CLUSTER.  Where there are more tiles than clusters, every block takes tiles of its
+// own; with fewer, the blocks of a cluster take a part of K each and add their sums up, always in the same order, through
+// each other's shared memory.  Clusters of two: 74 of them fit, clusters of four only on 132 of the 148 SMs, which
+// costs 32 groups of 8 rows (4096 x 7168) 104 us instead of 82.  Clusters of four where no more than 32 tiles can come:
+// one row, 4096 x 4096, 6.0 us instead of 7.4.
+namespace ff {
+constexpr int BKB = 128, THREADS = 256, ACCS = 2;
+constexpr int FOUR_MAX_TILES = 32;
+template <bool NV, int NT> struct Cfg {
+    static constexpr int SF_CHUNK = NV ? 2048 : 1024;
+    static constexpr int W_BYTES = 128 * BKB, X_BYTES = NT * BKB;
+    static constexpr int STAGE = W_BYTES + X_BYTES + 2 * SF_CHUNK;
+    static constexpr int STAGES = NT == 32 ? 4 : 5;
+    static constexpr int BLOCKS_PER_SM = NT == 32 ? 2 : 1;
+    static constexpr int SF_COLS = NV ? 16 : 8;                  // scale columns of one operand and stage
+    static constexpr int COLS = ACCS * NT + STAGES * 2 * SF_COLS, TMEM_COLS = COLS > 256 ? 512 : (COLS > 128 ? 256 : 128);
+    static constexpr int OFF_X = STAGES * W_BYTES;
+    static constexpr int OFF_SF = OFF_X + STAGES * X_BYTES;
+    static constexpr int OFF_BARS = OFF_SF + STAGES * 2 * SF_CHUNK;
+    static constexpr int OFF_LIST = OFF_BARS + 256;
+    static constexpr int SMEM_BYTES = OFF_LIST + gg::MAX_MASKED_GROUPS * 4 + 1024;
+    static_assert(COLS <= 512 && BLOCKS_PER_SM * TMEM_COLS <= 512, "accumulators and scales must fit TMEM");
+    static_assert(STAGES * STAGE >= NT * 128 * 4, "the ring's memory holds the sums of a cluster's blocks for one block's columns");
+};
+}  // namespace ff
+
+template <bool NV>
+__device__ __forceinline__ void umma_fp4(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t tmem_sfa, uint32_t tmem_sfb,
+                                         uint32_t accumulate) {
+    if (NV)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%5], [%6], p;\n\t}"
+            ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(tmem_sfa), "r"(tmem_sfb) : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n\t}"
+            ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(tmem_sfa), "r"(tmem_sfb) : "memory");
+}
+
+// 32 rows of one column of d: row j, where bit j of `rows` is set, at d + j * ldd
+template <typename T>
+__device__ __forceinline__ void few_store(T* d, long long ldd, unsigned rows, const uint32_t (&v)[32], float alpha) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j, d += ldd)
+        if ((rows >> j) & 1u) *d = from_f32<T>(__uint_as_float(v[j]) * alpha);
+}
+
+template <bool NV, int NT, int CLUSTER>
+__global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(ff::THREADS, 2)
+gg_fp4_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const GGFp4Params p, int x_box_rows,
+                  int* status) {
+    using namespace ff;
+    using C = Cfg<NV, NT>;
+    constexpr int STAGES = C::STAGES;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BARS);          // full[S], empty[S], tmem_full[2], tmem_empty[2]
+    uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 4);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_base_slot + 1);
+    int* list = reinterpret_cast<int*>(smem + C::OFF_LIST);                    // the groups that have rows
+    volatile int* list_len = reinterpret_cast<volatile int*>(tmem_base_slot + 2);
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const uint32_t full_bar = smem_u32(bars), empty_bar = smem_u32(bars + STAGES);
+    const uint32_t tfull_bar = smem_u32(bars + 2 * STAGES), tempty_bar = smem_u32(bars + 2 * STAGES + 2);
+    const int rows_end = !p.masked && p.rows_used ? min(p.M, __ldg(p.rows_used)) : p.M;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(full_bar + 8 * s, 1);
+            mbar_init(empty_bar + 8 * s, 1);
+        }
+        for (int a = 0; a < ACCS; ++a) {
+            mbar_init(tfull_bar + 8 * a, 1);
+            mbar_init(tempty_bar + 8 * a, 4);
+        }
+        *abort_flag = 0;
+        fence_mbar_init();
+        tma_prefetch_desc(&tmap_w);
+        tma_prefetch_desc(&tmap_x);
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_u32(tmem_base_slot), C::TMEM_COLS);
+        tmem_relinquish();
+    }
+    if (warp == 2) {
+        int n = 0;
+        if (p.masked) {
+            for (int base = 0; base < p.G; base += 32) {
+                const bool has = base + lane < p.G && __ldg(p.layout + base + lane) > 0;
+                const unsigned b = __ballot_sync(0xffffffffu, has);
+                if (has) list[n + __popc(b & ((1u << lane) - 1u))] = base + lane;
+                n += __popc(b);
+            }
+        } else {
+            // the distinct groups of the (at most NT) rows, ascending
+            int vals[NT / 32];
+#pragma unroll
+            for (int j = 0; j < NT / 32; ++j) {
+                const int r = lane + 32 * j;
+                vals[j] = r < rows_end ? __ldg(p.layout + r) : -1;
+            }
+            int after = -1;
+            while (true) {
+                int best = INT_MAX;
+#pragma unroll
+                for (int j = 0; j < NT / 32; ++j)
+                    if (vals[j] > after && vals[j] < p.G && vals[j] < best) best = vals[j];
+                best = __reduce_min_sync(0xffffffffu, best);
+                if (best == INT_MAX) break;
+                if (lane == 0) list[n] = best;
+                ++n;
+                after = best;
+            }
+        }
+        if (lane == 0) *list_len = n;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_base_slot;
+    const int KB = (p.K + 255) / 256, n_tiles = (p.N + 127) / 128;
+    const int tiles = *list_len * n_tiles, clusters = gridDim.x / CLUSTER;
+    const int rank = (int)cluster_ctarank(), cluster = blockIdx.x / CLUSTER;
+    // few tiles: one per cluster, a part of K per block; else one after the other per block, spread over the clusters first
+    const bool split = tiles <= clusters;
+    const int first = split ? cluster : rank * clusters + cluster, step = gridDim.x;
+    const int kb0 = split ? KB * rank / CLUSTER : 0, kb1 = split ? KB * (rank + 1) / CLUSTER : KB;
+
+    if (warp == 0) {
+        // ------------------------------------------------ producer
+        uint32_t stage = 0, phase = 0;
+        bool ok = true;
+        for (int t = first; ok && t < tiles; t += step) {
+            const int g = list[t / n_tiles], nt = t % n_tiles;
+            const int w_row = g * p.N + nt * 128, x_row = p.masked ? g * p.M : 0;
+            const uint8_t* sfw = p.sfb + ((long long)g * p.b_tiles + nt) * KB * C::SF_CHUNK;
+            const uint8_t* sfx = p.sfa + (p.masked ? (long long)g * p.a_tiles : 0) * KB * C::SF_CHUNK;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                ok = mbar_wait_warp(empty_bar + 8 * stage, phase ^ 1, abort_flag, status, STATUS_TIMEOUT_SMEM_EMPTY);
+                if (!ok) break;
+                if (elect_one_sync()) {
+                    const uint32_t fb = full_bar + 8 * stage, sf = smem_u32(smem + C::OFF_SF + stage * 2 * C::SF_CHUNK);
+                    mbar_arrive_expect_tx(fb, C::W_BYTES + x_box_rows * BKB + 2 * C::SF_CHUNK);
+                    tma_load_2d(smem_u32(smem + stage * C::W_BYTES), &tmap_w, fb, kb * BKB, w_row);
+                    tma_load_2d(smem_u32(smem + C::OFF_X + stage * C::X_BYTES), &tmap_x, fb, kb * BKB, x_row);
+                    bulk_load(sf, sfw + (long long)kb * C::SF_CHUNK, C::SF_CHUNK, fb);
+                    bulk_load(sf + C::SF_CHUNK, sfx + (long long)kb * C::SF_CHUNK, C::SF_CHUNK, fb);
+                }
+                if (++stage == STAGES) { stage = 0; phase ^= 1; }
+            }
+        }
+        if (!ok) {                // unwinding: copies in flight get time to land before the block's memory goes
+            const uint64_t t0 = globaltimer_ns();
+            while (globaltimer_ns() - t0 < 1000000ull) {}
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------ MMA issuer
+        uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
+        bool ok = true;
+        const uint64_t wdesc0 = make_smem_desc_sw128(smem_u32(smem)), xdesc0 = make_smem_desc_sw128(smem_u32(smem + C::OFF_X));
+        const uint64_t sdesc0 = make_sf_desc(smem_u32(smem + C::OFF_SF));
+        const uint32_t idesc = make_idesc_fp4<NV>(128, NT, 0);
+        for (int t = first; ok && t < tiles && kb0 < kb1; t += step) {
+            ok = mbar_wait_warp(tempty_bar + 8 * acc, acc_phase ^ 1, abort_flag, status, STATUS_TIMEOUT_TMEM_EMPTY);
+            if (!ok) break;
+            tc_fence_after();
+            for (int kb = kb0; kb < kb1; ++kb) {
+                ok = mbar_wait_warp(full_bar + 8 * stage, phase, abort_flag, status, STATUS_TIMEOUT_SMEM_FULL);
+                if (!ok) break;
+                tc_fence_after();
+                if (elect_one_sync()) {
+                    const uint32_t sfw = tmem_base + ACCS * NT + stage * 2 * C::SF_COLS, sfx = sfw + C::SF_COLS;
+                    const uint64_t sd = sdesc0 + stage * (2 * C::SF_CHUNK >> 4);
+#pragma unroll
+                    for (int j = 0; j < C::SF_COLS / 4; ++j) {
+                        tmem_cp_sf(sfw + 4 * j, sd + j * 32);
+                        tmem_cp_sf(sfx + 4 * j, sd + (C::SF_CHUNK >> 4) + j * 32);
+                    }
+                    const uint64_t wd = wdesc0 + stage * (C::W_BYTES >> 4), xd = xdesc0 + stage * (C::X_BYTES >> 4);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int w = NV ? j : j >> 1;
+                        const uint32_t id = NV ? 0u : (uint32_t)(j & 1) * 2u;
+                        umma_fp4<NV>(tmem_base + acc * NT, wd + 2 * j, xd + 2 * j, idesc | (id << 4) | (id << 29), sfw + 4 * w, sfx + 4 * w,
+                                     kb > kb0 || j > 0 ? 1u : 0u);
+                    }
+                    umma_commit(empty_bar + 8 * stage);
+                    if (kb == kb1 - 1) umma_commit(tfull_bar + 8 * acc);
+                }
+                if (++stage == STAGES) { stage = 0; phase ^= 1; }
+            }
+            if (++acc == ACCS) { acc = 0; acc_phase ^= 1; }
+        }
+    }
+    // ---------------------------------------------------- epilogue: thread = column of d, register = row
+    const int ew = warp - 4;                       // TMEM lane quarter (warp % 4)
+    // which of the 32 rows from row0 on belong to group g
+    auto rows_of = [&](int g, int row0) -> unsigned {
+        if (p.masked) {
+            const int left = min(p.M, __ldg(p.layout + g)) - row0;
+            return left >= 32 ? 0xffffffffu : (left > 0 ? (1u << left) - 1u : 0u);
+        }
+        return __ballot_sync(0xffffffffu, row0 + lane < rows_end && __ldg(p.layout + row0 + lane) == g);
+    };
+    auto alpha_of = [&](int g) { return p.alpha ? __ldg(p.alpha + g * p.alpha_stride) : 1.0f; };
+    if (warp >= 4 && !split) {
+        uint32_t acc = 0, acc_phase = 0;
+        for (int t = first; t < tiles; t += step) {
+            const int g = list[t / n_tiles], n = (t % n_tiles) * 128 + ew * 32 + lane;
+            const float alpha = alpha_of(g);
+            if (!mbar_wait_warp(tfull_bar + 8 * acc, acc_phase, abort_flag, status, STATUS_TIMEOUT_TMEM_FULL)) break;
+            tc_fence_after();
+            long long o = (p.masked ? (long long)g * p.M * p.ldd : 0) + n;
+#pragma unroll 1
+            for (int w = 0; w < NT; w += 32, o += 32 * p.ldd) {
+                unsigned rows = rows_of(g, w);
+                uint32_t v[32];
+                if (rows != 0u) {
+                    tmem_ld_32x32b_x32(tmem_base + (uint32_t(ew * 32) << 16) + acc * NT + w, v);
+                    tmem_ld_wait(v);
+                }
+                if (w == NT - 32) {            // the accumulator is in registers
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(tempty_bar + 8 * acc);
+                }
+                if (n >= p.N) rows = 0u;
+                if (p.d_f32) few_store(static_cast<float*>(p.d) + o, p.ldd, rows, v, alpha);
+                else few_store(static_cast<__nv_bfloat16*>(p.d) + o, p.ldd, rows, v, alpha);
+            }
+            if (++acc == ACCS) { acc = 0; acc_phase ^= 1; }
+        }
+    }
+    if (split) {
+        constexpr int F = 128 / CLUSTER;           // columns that a block finishes
+        const bool work = first < tiles;
+        const int g = work ? list[first / n_tiles] : 0, n0 = work ? (first % n_tiles) * 128 : 0, c = ew * 32 + lane;
+        if (warp >= 4 && work && kb0 < kb1) mbar_wait_warp(tfull_bar, 0, abort_flag, status, STATUS_TIMEOUT_TMEM_FULL);
+        __syncwarp();
+        // every block of the cluster has read all of its stages: their memory takes the sums, [rank][row][F columns]
+        cluster_sync_all();
+        if (warp >= 4 && work) {
+            tc_fence_after();
+            const uint32_t dst = map_to_cta(smem_u32(smem), c / F) + (rank * NT * F + c % F) * 4;
+#pragma unroll 1
+            for (int w = 0; w < NT; w += 32) {
+                const unsigned rows = rows_of(g, w);
+                if (rows == 0u) continue;
+                uint32_t v[32];
+                tmem_ld_32x32b_x32(tmem_base + (uint32_t(ew * 32) << 16) + w, v);
+                tmem_ld_wait(v);
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    if ((rows >> j) & 1u)
+                        asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(dst + (w + j) * F * 4), "r"(kb0 < kb1 ? v[j] : 0u) : "memory");
+            }
+        }
+        __syncwarp();
+        cluster_sync_all();
+        if (warp >= 4 && work) {
+            const float alpha = alpha_of(g);
+            const int n = n0 + rank * F + c % F;
+            const float* part = reinterpret_cast<const float*>(smem) + c % F;
+#pragma unroll 1
+            for (int w = 0; w < NT; w += 32) {
+                const unsigned rows = rows_of(g, w);
+                for (int j = c / F; j < 32; j += CLUSTER)
+                    if (((rows >> j) & 1u) && n < p.N) {
+                        float v = part[(w + j) * F];
+#pragma unroll
+                        for (int r = 1; r < CLUSTER; ++r) v += part[(r * NT + w + j) * F];
+                        const long long o = ((p.masked ? (long long)g * p.M : 0) + w + j) * p.ldd + n;
+                        if (p.d_f32) static_cast<float*>(p.d)[o] = v * alpha;
+                        else static_cast<__nv_bfloat16*>(p.d)[o] = __float2bfloat16_rn(v * alpha);
+                    }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, C::TMEM_COLS);
+    }
+}
+
 }  // namespace b200

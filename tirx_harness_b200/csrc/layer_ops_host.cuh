@@ -197,6 +197,31 @@ int launch_fp4_pair_layout(const GGFp4Params& p, long long rows_total, DeviceInf
     return p.masked ? launch_fp4_pair<NV, true, TN>(p, rows_total, di, st) : launch_fp4_pair<NV, false, TN>(p, rows_total, di, st);
 }
 
+template <bool NV, int NT, int CLUSTER>
+int launch_fp4_few_clusters(const GGFp4Params& p, long long rows_total, long long tiles, DeviceInfo* di, cudaStream_t st) {
+    using C = ff::Cfg<NV, NT>;
+    CUtensorMap tw, tx;
+    int rc;
+    // no more rows than there are: the others of the stage keep whatever it held, and their products are not stored
+    const int box = NT > 32 ? NT : (p.M <= 8 ? 8 : (p.M <= 16 ? 16 : 32));
+    if ((rc = encode_fp8_kmajor(&tw, p.b, (uint64_t)p.G * p.N, (uint64_t)p.K / 2, 128)) != MOE_OK) return rc;
+    if ((rc = encode_fp8_kmajor(&tx, p.a, (uint64_t)rows_total, (uint64_t)p.K / 2, box)) != MOE_OK) return rc;
+    static std::atomic<uint64_t> done{0};
+    if ((rc = raise_smem(gg_fp4_few_kernel<NV, NT, CLUSTER>, C::SMEM_BYTES, done)) != MOE_OK) return rc;
+    const long long fit = (long long)C::BLOCKS_PER_SM * di->num_sms / CLUSTER;
+    const int clusters = (int)(tiles < fit ? tiles : fit);
+    gg_fp4_few_kernel<NV, NT, CLUSTER><<<clusters * CLUSTER, ff::THREADS, C::SMEM_BYTES, st>>>(tw, tx, p, box, di->status);
+    CUDA_TRY(cudaGetLastError());
+    return MOE_OK;
+}
+template <bool NV, int NT>
+int launch_fp4_few(const GGFp4Params& p, long long rows_total, DeviceInfo* di, cudaStream_t st) {
+    // the most tiles that can come: the groups with rows are known on the device only
+    const long long tiles = (long long)(p.masked || p.G < p.M ? p.G : p.M) * ((p.N + 127) / 128);
+    return tiles <= ff::FOUR_MAX_TILES ? launch_fp4_few_clusters<NV, NT, 4>(p, rows_total, tiles, di, st)
+                                       : launch_fp4_few_clusters<NV, NT, 2>(p, rows_total, tiles, di, st);
+}
+
 int launch_gg_fp4(const moe_gg_fp4_args* a, bool masked, void* stream) {
     if (!a) return fail(MOE_ERR_INVALID, "args is NULL");
     if (a->G <= 0 || a->N <= 0 || a->K <= 0 || a->M < 0)
@@ -229,7 +254,10 @@ int launch_gg_fp4(const moe_gg_fp4_args* a, bool masked, void* stream) {
     p.kt = (a->K + 255) / 256 * (a->format == MOE_FP4_NV ? 4 : 2);
     p.a_tiles = (a->M + 127) / 128; p.b_tiles = (a->N + 127) / 128;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return a->format == MOE_FP4_NV ? launch_fp4_pair_layout<true, 256>(p, rows_total, di, st) : launch_fp4_pair_layout<false, 256>(p, rows_total, di, st);
+    const bool nv = a->format == MOE_FP4_NV;
+    if (a->M <= 32) return nv ? launch_fp4_few<true, 32>(p, rows_total, di, st) : launch_fp4_few<false, 32>(p, rows_total, di, st);
+    if (a->M <= 128) return nv ? launch_fp4_few<true, 128>(p, rows_total, di, st) : launch_fp4_few<false, 128>(p, rows_total, di, st);
+    return nv ? launch_fp4_pair_layout<true, 256>(p, rows_total, di, st) : launch_fp4_pair_layout<false, 256>(p, rows_total, di, st);
 }
 
 }  // namespace
