@@ -582,12 +582,28 @@ def test_product_contiguous(gg, rows, pads, N, K, fmt, dtype):
     check_product(d2, torch.full_like(d2, 3.0), av, bv, half, alpha[:1], DT[dtype])
 
 
-def test_product_rows_in_any_order(gg):
-    layout = torch.randint(-1, 3, (300,), generator=gen(32)).int()
-    a, sfa, av = make_operand((), 300, 256, "nvfp4", 33)
-    b, sfb, bv = make_operand((3,), 136, 256, "nvfp4", 34)
-    d = torch.zeros((300, 136), dtype=torch.bfloat16, device="cuda")
+@pytest.mark.parametrize("M,G,low", [(300, 3, -1), (1500, 150, 0), (90, 5, -1), (700, 4, -300)])
+def test_product_rows_in_any_order(gg, M, G, low):
+    """Several groups in every block of rows, in no order; 1500 rows of 150 groups are more than the list of blocks holds."""
+    layout = torch.randint(low, G, (M,), generator=gen(32)).int()
+    layout[M // 3] = G + 5                                # no such group: a padding row
+    a, sfa, av = make_operand((), M, 256, "nvfp4", 33)
+    b, sfb, bv = make_operand((G,), 136, 256, "nvfp4", 34)
+    d = torch.zeros((M, 136), dtype=torch.bfloat16, device="cuda")
     gg.bind_contiguous_fp4(a, sfa, b, sfb, d, layout.cuda())()
+    assert gg.device_status() == 0
+    layout[M // 3] = -1
+    check_product(d, torch.zeros_like(d), av, bv, layout, None, torch.bfloat16)
+
+
+def test_product_more_row_blocks_than_the_list_holds(gg):
+    """131073 rows and more: 1025 blocks of 128."""
+    M, N, K = 131072 + 300, 64, 128
+    layout = torch.arange(M, dtype=torch.int32) // 70000
+    a, sfa, av = make_operand((), M, K, "mxfp4", 35)
+    b, sfb, bv = make_operand((2,), N, K, "mxfp4", 36)
+    d = torch.zeros((M, N), dtype=torch.bfloat16, device="cuda")
+    gg.bind_contiguous_fp4(a, sfa, b, sfb, d, layout.cuda(), fmt="mxfp4")()
     check_product(d, torch.zeros_like(d), av, bv, layout, None, torch.bfloat16)
 
 

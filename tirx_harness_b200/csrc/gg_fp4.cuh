@@ -77,6 +77,139 @@ template <bool NV, int TN> struct Cfg {
 };
 }  // namespace f4
 
+// ---- schedule of the contiguous layout: which two 128-row blocks a pair multiplies at a time
+// PairScheduler (pair_common.cuh) cuts the rows into fixed blocks of 256 and visits each once per group found in it, so that
+// a group that begins in the middle of one costs a tile more.  Here the blocks of 128 rows are listed with the groups found in
+// them, and neighbouring blocks of one group are paired from its first one on.  A last block without a partner leaves the
+// second half of the tile empty: its rows are fetched from behind the matrix, which reads as zeros and moves no data.
+// Up to 1024 (block, group) entries, built by every block for itself (M layout entries read once); larger ones and
+// layouts with more groups per block take PairScheduler.
+// 28672 rows in 32 ragged groups (4096 x 7168): 438 us with fixed blocks, 382 us paired.
+constexpr int PAIR_LIST_CAP = 1024, PAIR_LIST_BLOCK_BITS = 11, PAIR_LIST_MAX_G = 1 << 20;
+
+// list[i] = first block | group << 11 | (two blocks) << 31; returns the number of tiles, -1: too many.  Called by the whole
+// block; `scratch`: 3 * 1024 ints.
+__device__ __forceinline__ int build_pair_list(const GGFp4Params& p, int* list, int* scratch) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    const int rows_end = p.rows_used ? min(p.M, max(0, __ldg(p.rows_used))) : p.M;
+    const int nb = (rows_end + 127) >> 7;
+    if (nb > PAIR_LIST_CAP || p.G > PAIR_LIST_MAX_G) return -1;
+    int* count = scratch;                            // groups in a block
+    int* lowest = scratch + PAIR_LIST_CAP;           // the first of them, then where the block's entries begin
+    int* entry = scratch + 2 * PAIR_LIST_CAP;        // block | group << 11
+    auto load = [&](int b, int (&v)[4]) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int r = b * 128 + j * 32 + lane;
+            v[j] = r < rows_end ? __ldg(p.layout + r) : -1;
+            if (v[j] < 0 || v[j] >= p.G) v[j] = INT_MAX;
+        }
+    };
+    auto after = [&](const int (&v)[4], int g) {     // the lowest group above g, INT_MAX: none
+        int m = INT_MAX;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) if (v[j] > g) m = min(m, v[j]);
+        return __reduce_min_sync(0xffffffffu, m);
+    };
+#pragma unroll 2
+    for (int b = warp; b < nb; b += warps) {
+        int v[4];
+        load(b, v);
+        int g = after(v, -1), n = 0;
+        const int first = g;
+        while (g != INT_MAX) { ++n; g = after(v, g); }
+        if (lane == 0) { count[b] = n; lowest[b] = first; }
+    }
+    __syncthreads();
+    int total = 0;                                   // the same in every warp
+    for (int base = 0; base < nb; base += 32) {
+        const int n = base + lane < nb ? count[base + lane] : 0;
+        int incl = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += u;
+        }
+        // warp w writes the entries of the blocks w, w + warps, ..: a block with one group at once
+        for (unsigned todo = __ballot_sync(0xffffffffu, base + lane < nb && n > 0 && (base + lane) % warps == warp); todo; todo &= todo - 1) {
+            const int i = __ffs(todo) - 1, b = base + i;
+            int at = total + __shfl_sync(0xffffffffu, incl - n, i);
+            const int m = __shfl_sync(0xffffffffu, n, i);
+            if (at + m > PAIR_LIST_CAP) continue;
+            if (m == 1) {
+                if (lane == 0) entry[at] = b | lowest[b] << PAIR_LIST_BLOCK_BITS;
+            } else {
+                int v[4];
+                load(b, v);
+                for (int g = after(v, -1); g != INT_MAX; g = after(v, g), ++at)
+                    if (lane == 0) entry[at] = b | g << PAIR_LIST_BLOCK_BITS;
+            }
+        }
+        total += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    __syncthreads();
+    if (total > PAIR_LIST_CAP) return -1;
+    // pairs: an entry continues the one before if it is the next block of the same group; every second one of such a run begins a
+    // tile.  Each warp works the whole list out, warp 0 writes it.
+    int tiles = 0, run = 0;                          // run: where the run of the last entry so far begins
+    for (int base = 0; base < total; base += 32) {
+        const int i = base + lane;
+        const bool in = i < total;
+        const int e = in ? entry[i] : -1;
+        const bool cont = in && i > 0 && entry[i - 1] + 1 == e;
+        int start = in && !cont ? i : run;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, start, o);
+            if (lane >= o) start = max(start, u);
+        }
+        run = __shfl_sync(0xffffffffu, start, 31);
+        const bool head = in && ((i - start) & 1) == 0;
+        const unsigned heads = __ballot_sync(0xffffffffu, head);
+        if (warp == 0 && head) {
+            const bool two = i + 1 < total && e + 1 == entry[i + 1];
+            list[tiles + __popc(heads & ((1u << lane) - 1u))] = (int)((uint32_t)e | (two ? 0x80000000u : 0u));
+        }
+        tiles += __popc(heads);
+    }
+    return tiles;
+}
+
+// Walks the list, columns fastest, like PairScheduler.
+struct PairListScheduler {
+    const GGFp4Params& p;
+    const int* list;
+    int t, total, n_blocks, stride, rank;
+    __device__ __forceinline__ PairListScheduler(const GGFp4Params& p_, const int* list_, int tiles, int n_blocks_, int rank_)
+        : p(p_), list(list_), t(blockIdx.x >> 1), total(tiles * n_blocks_), n_blocks(n_blocks_), stride(gridDim.x >> 1), rank(rank_) {}
+    __device__ __forceinline__ bool next(Tile& tile) {
+        if (t >= total) return false;
+        const uint32_t e = (uint32_t)list[t / n_blocks];
+        const int b = (int)(e & ((1u << PAIR_LIST_BLOCK_BITS) - 1u));
+        tile.g = (int)((e & 0x7FFFFFFFu) >> PAIR_LIST_BLOCK_BITS);
+        tile.n_blk = t % n_blocks;
+        tile.m0 = (rank == 0 || (e & 0x80000000u) ? b + rank : p.a_tiles) * 128;
+        tile.rows = 128;
+        t += stride;
+        return true;
+    }
+};
+
+// One of the two schedules, decided per launch and block alike.
+template <bool MASKED> struct Fp4Sched {
+    bool listed;
+    PairListScheduler l;
+    PairScheduler<MASKED> s;
+    __device__ __forceinline__ Fp4Sched(const GGFp4Params& p, const GGParams& sp, const int* table, int tiles, int lane, int rank)
+        : listed(!MASKED && tiles >= 0), l(p, table, tiles, sp.num_n_blocks, rank), s(sp, table, lane, rank) {}
+    __device__ __forceinline__ bool next(Tile& tile) {
+        if (listed) return l.next(tile);
+        if (!s.next(tile)) return false;
+        if (MASKED && tile.rows == 0) tile.m0 = l.p.G * l.p.M;        // nothing in this half: read zeros from behind the matrix
+        return true;
+    }
+};
+
 template <bool NV, bool MASKED, int TN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(f4::THREADS, 1)
 gg_fp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
@@ -137,6 +270,11 @@ gg_fp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
         tmem_alloc_pair(smem_u32(tmem_base_slot), TMEM_COLS);
         tmem_relinquish_pair();
     }
+    int listed_tiles = -1;
+    if (!MASKED) {
+        listed_tiles = build_pair_list(p, prefix, reinterpret_cast<int*>(smem));
+        fence_proxy_async_smem();                 // the ring's memory served as scratch; bulk copies write it from here on
+    }
     tc_fence_before();
     __syncthreads();
     cluster_sync_all();
@@ -151,15 +289,15 @@ gg_fp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
         setmaxnreg_dec<72>();
         if (warp == 0) {
             // ------------------------------------------------ TMA producer (both CTAs)
-            PairScheduler<MASKED> sched(sp, prefix, lane, rank);
+            Fp4Sched<MASKED> sched(p, sp, prefix, listed_tiles, lane, rank);
             Tile tile;
             uint32_t stage = 0, phase = 0;
             bool ok = true;
             while (ok && sched.next(tile)) {
                 const int n0 = tile.n_blk * TN;
                 const int b_row = tile.g * p.N + n0 + (int)rank * (tile_cols(tile.n_blk) >> 1);
-                const int row = MASKED ? tile.m0 - tile.g * p.M : tile.m0;
-                const int a_blk = (MASKED ? tile.g * p.a_tiles : 0) + (row >> 7), b_blk = tile.g * p.b_tiles + (n0 >> 7);
+                const int a_blk = !MASKED ? tile.m0 >> 7 : (tile.rows == 0 ? p.G * p.a_tiles : tile.g * p.a_tiles + ((tile.m0 - tile.g * p.M) >> 7));
+                const int b_blk = tile.g * p.b_tiles + (n0 >> 7);
                 for (int kb = 0; kb < KB; ++kb) {
                     ok = mbar_wait_warp(empty_bar + 8 * stage, phase ^ 1, abort_flag, status, STATUS_TIMEOUT_SMEM_EMPTY);
                     if (!ok) break;
@@ -183,7 +321,7 @@ gg_fp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
             }
         } else if (warp == 1 && rank == 0) {
             // ------------------------------------------------ MMA issuer (leader)
-            PairScheduler<MASKED> sched(sp, prefix, lane, rank);
+            Fp4Sched<MASKED> sched(p, sp, prefix, listed_tiles, lane, rank);
             Tile tile, next_tile;
             uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0, sfb_buf = 0;
             bool ok = true;
@@ -240,7 +378,7 @@ gg_fp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
         const int quarter = warp & 3, half = (warp - 4) >> 2;
         const int row_in_tile = quarter * 32 + lane;
         const int m_end = !MASKED && p.rows_used ? min(p.M, __ldg(p.rows_used)) : p.M;       // rows behind it are not written
-        PairScheduler<MASKED> sched(sp, prefix, lane, rank);
+        Fp4Sched<MASKED> sched(p, sp, prefix, listed_tiles, lane, rank);
         Tile tile;
         uint32_t acc = 0, acc_phase = 0;
         bool ok = true;
