@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libb200moe.so")
@@ -214,6 +215,53 @@ def set_option(option: int, value: int) -> int:
     check(lib().moe_get_option(ctypes.c_int32(option), ctypes.byref(old)))
     check(lib().moe_set_option(ctypes.c_int32(option), ctypes.c_int32(value)))
     return old.value
+
+
+class Entry:
+    """An entry point that takes one argument block and a stream.  ``pack`` lays a block's values out as bytes in the order
+    of the structure's fields (pointers as integers, 0 = NULL), several times faster than filling a ctypes structure: a
+    call that launches one small kernel costs the host more than the GPU."""
+
+    _CODES = {_c.c_void_p: "P", _c.c_int64: "q", _c.c_uint64: "Q", _c.c_int32: "i", _c.c_float: "f"}
+    _ARGTYPES = (_c.c_char_p, _c.c_void_p)
+
+    def __init__(self, name: str, args):
+        layout = struct.Struct("@" + "".join(self._CODES[t] for _, t in args._fields_) + "0P")
+        assert layout.size == _c.sizeof(args), name
+        self.pack, self._name, self._fn = layout.pack, name, None
+
+    def _bind(self):
+        self._fn = _c.CFUNCTYPE(_c.c_int, *self._ARGTYPES)((self._name, lib()))
+        return self._fn
+
+    def __call__(self, block: bytes, stream: int) -> None:
+        rc = (self._fn or self._bind())(block, stream)
+        if rc != 0:
+            check(rc)
+
+
+class UnpackEntry(Entry):
+    """moe_unpack_fp4: pointers and a size instead of a block."""
+
+    _ARGTYPES = (_c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_void_p)
+
+    def __init__(self, name: str):
+        self.pack, self._name, self._fn = (lambda *values: values), name, None
+
+    def __call__(self, values, stream: int) -> None:
+        rc = (self._fn or self._bind())(*values, stream)
+        if rc != 0:
+            check(rc)
+
+
+NORM = Entry("moe_rms_norm_quant", NormArgs)
+NORM_GRAD = Entry("moe_rms_norm_backward", NormGradArgs)
+ROUTE = Entry("moe_route", RouteArgs)
+ROUTE_GRAD = Entry("moe_route_backward", RouteGradArgs)
+UNPACK_FP4 = UnpackEntry("moe_unpack_fp4")
+FP4_QUANT = Entry("moe_quant_fp4", Fp4QuantArgs)
+GG_FP4_CONTIGUOUS = Entry("moe_gg_fp4_contiguous", GGFp4Args)
+GG_FP4_MASKED = Entry("moe_gg_fp4_masked", GGFp4Args)
 
 
 def check(rc: int) -> None:

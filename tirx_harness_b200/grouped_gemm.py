@@ -239,21 +239,17 @@ def bind_k_grouped(a, sfa_words, b, sfb_words, d, ks) -> _BoundKGrouped:
 class _BoundFp4:
     """4-bit grouped GEMM bound to its tensors; ``__call__`` launches on the current stream of their device."""
 
-    def __init__(self, fn_name, a, sfa, b, sfb, d, layout, alpha, fmt, G, M, N, K, rows_used=None):
+    def __init__(self, entry, a, sfa, b, sfb, d, layout, alpha, fmt, G, M, N, K, rows_used=None):
         self._keep = (a, sfa, b, sfb, d, layout, alpha, rows_used)
-        self._fn = getattr(_lib.lib(), fn_name)
-        self._device = d.device
-        self._args = _lib.GGFp4Args(
-            a=_ptr(a), sfa=_ptr(sfa), b=_ptr(b), sfb=_ptr(sfb), alpha=_ptr(alpha) if alpha is not None else None,
-            alpha_stride=1 if alpha is not None and alpha.numel() > 1 else 0, layout=_ptr(layout),
-            rows_used=_ptr(rows_used) if rows_used is not None else None, d=_ptr(d), ldd=max(d.stride(-2), N), G=G, M=M, N=N, K=K,
-            format=moe_ops._FP4_FORMAT[fmt], d_dtype=1 if d.dtype == torch.float32 else 0)
-        self.out = d
+        self._entry, self._device, self.out = entry, d.device, d
+        ldd = d.stride(-2) if M > 1 else (N + 7) // 8 * 8
+        self._values = (a.data_ptr(), sfa.data_ptr(), b.data_ptr(), sfb.data_ptr(), 0 if alpha is None else alpha.data_ptr(),
+                        1 if alpha is not None and alpha.numel() > 1 else 0, layout.data_ptr(),
+                        0 if rows_used is None else rows_used.data_ptr(), d.data_ptr(), ldd, G, M, N, K, moe_ops._FP4_FORMAT[fmt],
+                        1 if d.dtype == torch.float32 else 0)
 
     def __call__(self):
-        with torch.cuda.device(self._device):
-            stream = torch.cuda.current_stream().cuda_stream
-            _lib.check(self._fn(ctypes.byref(self._args), ctypes.c_void_p(stream)))
+        moe_ops._launch(self._entry, self._device, *self._values)
         return self.out
 
 
@@ -293,7 +289,7 @@ def bind_contiguous_fp4(a, sfa, b, sfb, d, grouped_layout, alpha=None, fmt: str 
         raise ValueError(f"grouped_layout must be int32 [{M}]")
     if rows_used is not None and (rows_used.dtype != torch.int32 or rows_used.device != b.device):
         raise ValueError(f"rows_used must be an int32 tensor on {b.device}")
-    return _BoundFp4("moe_gg_fp4_contiguous", a, sfa, b, sfb, d, grouped_layout, alpha, fmt, G, M, N, K, rows_used)
+    return _BoundFp4(_lib.GG_FP4_CONTIGUOUS, a, sfa, b, sfb, d, grouped_layout, alpha, fmt, G, M, N, K, rows_used)
 
 
 def bind_masked_fp4(a, sfa, b, sfb, d, masked_m, alpha=None, fmt: str = "nvfp4") -> _BoundFp4:
@@ -307,7 +303,7 @@ def bind_masked_fp4(a, sfa, b, sfb, d, masked_m, alpha=None, fmt: str = "nvfp4")
         raise ValueError(f"a and masked_m must have {G} groups")
     if d.dtype not in (torch.bfloat16, torch.float32) or tuple(d.shape) != (G, M, N) or not d.is_contiguous() or d.device != b.device:
         raise ValueError(f"d must be contiguous bfloat16 (or float32) [{G}, {M}, {N}] on {b.device}")
-    return _BoundFp4("moe_gg_fp4_masked", a, sfa, b, sfb, d, masked_m, alpha, fmt, G, M, N, K)
+    return _BoundFp4(_lib.GG_FP4_MASKED, a, sfa, b, sfb, d, masked_m, alpha, fmt, G, M, N, K)
 
 
 def m_grouped_fp8_gemm_nt_contiguous(a, sfa, b, sfb, d, grouped_layout):

@@ -138,10 +138,10 @@ _FP4_FORMAT = {"nvfp4": _lib.FP4_NV, "mxfp4": _lib.FP4_MX}
 
 
 def _p(t):
-    return t.data_ptr() if t is not None else None
+    return 0 if t is None else t.data_ptr()
 
 
-def _check_float(t, name, dtypes=tuple(_DTYPE)):
+def _check_float(t, name, dtypes=_DTYPE):
     if t.dtype not in dtypes:
         raise TypeError(f"{name} must be one of {', '.join(str(d)[6:] for d in dtypes)}, got {t.dtype}")
     if not t.is_cuda:
@@ -151,7 +151,7 @@ def _check_float(t, name, dtypes=tuple(_DTYPE)):
 def _check_like(t, name, shape, dtype, device, contiguous=True):
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, the other tensors on {device}")
@@ -159,18 +159,29 @@ def _check_like(t, name, shape, dtype, device, contiguous=True):
         raise ValueError(f"{name} must be contiguous")
 
 
-def _row_stride(t, name):
-    """Elements between the rows of a 2-d tensor whose columns are next to one another."""
+def _rows(t, name, step=8):
+    """(rows, columns, elements between rows) of a 2-d tensor whose columns are next to one another; a single row's distance
+    does not matter and is given as one that its columns and ``step`` allow."""
     if t.dim() != 2:
         raise ValueError(f"{name} must have two dimensions, got {t.dim()}")
-    if t.shape[1] != 1 and t.stride(1) != 1:
+    (n, cols), (ld, unit) = t.shape, t.stride()
+    if unit != 1 and cols > 1:
         raise ValueError(f"{name} must have unit column stride")
-    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], t.stride(0) // 8 * 8)
+    return n, cols, ld if n > 1 else (cols + step - 1) // step * step
 
 
-def _launch(fn_name, args, device):
-    with torch.cuda.device(device):
-        _lib.check(getattr(_lib.lib(), fn_name)(ctypes.byref(args), _vp(torch.cuda.current_stream(device).cuda_stream)))
+# the current stream of a device as an integer, without the object that torch.cuda.current_stream makes
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _launch(entry, device, *values):
+    """Calls an entry point on the current stream of the tensors' device, which need not be the current one."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        entry(entry.pack(*values), _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            entry(entry.pack(*values), _raw_stream(index))
 
 
 def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-6,
@@ -183,25 +194,26 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor
     :func:`quant_1x128` does it, from y in fp32.  ``pow2`` rounds the scales up to powers of two, which the grouped GEMM
     applies inside the tensor core; ``mn_major`` stores them [H/128, T].  H % 8 == 0, H <= 16384."""
     _check_float(x, "x")
-    ld = _row_stride(x, "x")
-    T, H = x.shape
-    if weight.dtype not in (x.dtype, torch.float32):
-        raise TypeError(f"weight must be {x.dtype} or float32, got {weight.dtype}")
-    _check_like(weight, "weight", (H,), weight.dtype, x.device)
-    ldr = 0
+    T, H, ld = _rows(x, "x")
+    dt, dev = x.dtype, x.device
+    if weight.dtype != dt and weight.dtype != torch.float32:
+        raise TypeError(f"weight must be {dt} or float32, got {weight.dtype}")
+    _check_like(weight, "weight", (H,), weight.dtype, dev)
+    ldr, h, y = 0, x, None
     if residual is not None:
-        _check_like(residual, "residual", (T, H), x.dtype, x.device, contiguous=False)
-        ldr = _row_stride(residual, "residual")
-    q = torch.empty((T, H), dtype=torch.float8_e4m3fn, device=x.device)
-    s = _scale_out(T, (H + 127) // 128, mn_major, x.device)
-    h = torch.empty((T, H), dtype=x.dtype, device=x.device) if residual is not None else x
-    y = torch.empty((T, H), dtype=x.dtype, device=x.device) if want_y else None
-    rstd = torch.empty(T, dtype=torch.float32, device=x.device)
-    _launch("moe_rms_norm_quant", _lib.NormArgs(
-        x=_p(x), x_stride=ld, residual=_p(residual), residual_stride=ldr, weight=_p(weight), q=_p(q), scales=_p(s),
-        ss_row=s.stride(0), ss_blk=s.stride(1), h=_p(h) if residual is not None else None, y=_p(y), rstd=_p(rstd), T=T, H=H,
-        dtype=_DTYPE[x.dtype], w_dtype=_DTYPE[weight.dtype], pow2=1 if pow2 else 0, eps=eps), x.device)
-    return dict(q=q, scales=s, h=h, y=y, rstd=rstd)
+        _check_like(residual, "residual", x.shape, dt, dev, contiguous=False)
+        ldr = _rows(residual, "residual")[2]
+        h = torch.empty_like(x, memory_format=torch.contiguous_format)
+    if want_y:
+        y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    nb = (H + 127) // 128
+    q = torch.empty_like(x, dtype=torch.float8_e4m3fn, memory_format=torch.contiguous_format)
+    s = x.new_empty((nb, T) if mn_major else (T, nb), dtype=torch.float32)
+    rstd = x.new_empty(T, dtype=torch.float32)
+    _launch(_lib.NORM, dev, x.data_ptr(), ld, _p(residual), ldr, weight.data_ptr(), q.data_ptr(), s.data_ptr(),
+            1 if mn_major else nb, T if mn_major else 1, h.data_ptr() if residual is not None else 0, _p(y), rstd.data_ptr(),
+            T, H, _DTYPE[dt], _DTYPE[weight.dtype], 1 if pow2 else 0, eps)
+    return dict(q=q, scales=s.t() if mn_major else s, h=h, y=y, rstd=rstd)
 
 
 def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor,
@@ -211,28 +223,27 @@ def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, r
     dy = dL/dy and h [T, H] of one type, rstd from the forward call, dh (optional) the gradient that reaches h past the
     norm -> (dx [T, H], the gradient of x and of residual alike; dw f32 [H])."""
     _check_float(dy, "dy")
-    ld = _row_stride(dy, "dy")
-    T, H = dy.shape
-    _check_like(h, "h", (T, H), dy.dtype, dy.device, contiguous=False)
-    if weight.dtype not in (dy.dtype, torch.float32):
-        raise TypeError(f"weight must be {dy.dtype} or float32, got {weight.dtype}")
-    _check_like(weight, "weight", (H,), weight.dtype, dy.device)
-    _check_like(rstd, "rstd", (T,), torch.float32, dy.device)
+    T, H, ld = _rows(dy, "dy")
+    dt, dev = dy.dtype, dy.device
+    _check_like(h, "h", dy.shape, dt, dev, contiguous=False)
+    if weight.dtype != dt and weight.dtype != torch.float32:
+        raise TypeError(f"weight must be {dt} or float32, got {weight.dtype}")
+    _check_like(weight, "weight", (H,), weight.dtype, dev)
+    _check_like(rstd, "rstd", (T,), torch.float32, dev)
     ldd = 0
     if dh is not None:
-        _check_like(dh, "dh", (T, H), dy.dtype, dy.device, contiguous=False)
-        ldd = _row_stride(dh, "dh")
-    dx = torch.empty((T, H), dtype=dy.dtype, device=dy.device)
-    dw = torch.empty(H, dtype=torch.float32, device=dy.device)
+        _check_like(dh, "dh", dy.shape, dt, dev, contiguous=False)
+        ldd = _rows(dh, "dh")[2]
+    dx = torch.empty_like(dy, memory_format=torch.contiguous_format)
+    dw = dy.new_empty(H, dtype=torch.float32)
     n = _lib.lib().moe_rms_norm_backward_workspace_bytes(_i32(T), _i32(H))
-    ws = torch.empty(n, dtype=torch.uint8, device=dy.device)
-    _launch("moe_rms_norm_backward", _lib.NormGradArgs(
-        dy=_p(dy), dy_stride=ld, h=_p(h), h_stride=_row_stride(h, "h"), weight=_p(weight), rstd=_p(rstd), dh=_p(dh), dh_stride=ldd,
-        dx=_p(dx), dw=_p(dw), T=T, H=H, dtype=_DTYPE[dy.dtype], w_dtype=_DTYPE[weight.dtype], workspace=_p(ws), workspace_bytes=n),
-        dy.device)
+    ws = dy.new_empty(n, dtype=torch.uint8)
+    _launch(_lib.NORM_GRAD, dev, dy.data_ptr(), ld, h.data_ptr(), _rows(h, "h")[2], weight.data_ptr(), rstd.data_ptr(), _p(dh), ldd,
+            dx.data_ptr(), dw.data_ptr(), T, H, _DTYPE[dt], _DTYPE[weight.dtype], ws.data_ptr(), n)
     return dx, dw
 
 
+_BIAS_DTYPE = (torch.bfloat16, torch.float32)
 _SCORE = {"softmax": 0, "sigmoid": 1}
 _GROUP_SCORE = {"max": 0, "top2": 1}
 
@@ -253,21 +264,17 @@ def route(logits: torch.Tensor, top_k: int, score: str = "softmax", bias: torch.
     sum of its two best ("top2").  A logit of -inf or NaN switches its expert off; where fewer than top_k are left the id
     is -1 and the weight 0, which :func:`permute_plan` drops."""
     _check_float(logits, "logits")
-    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
-        raise ValueError("logits must be [T, E] with unit column stride")
-    T, E = logits.shape
+    T, E, ld = _rows(logits, "logits", 1)
     if bias is not None:
-        _check_float(bias, "bias", (torch.bfloat16, torch.float32))
+        _check_float(bias, "bias", _BIAS_DTYPE)
         _check_like(bias, "bias", (E,), bias.dtype, logits.device)
     if not 0 < top_k <= min(32, E):
         raise ValueError(f"top_k must be in [1, min(32, E)], got {top_k}")
-    ids = torch.empty((T, top_k), dtype=torch.int32, device=logits.device)
-    w = torch.empty((T, top_k), dtype=torch.float32, device=logits.device)
-    _launch("moe_route", _lib.RouteArgs(
-        logits=_p(logits), stride=max(logits.stride(0), E) if T < 2 else logits.stride(0), bias=_p(bias), ids=_p(ids), weights=_p(w),
-        T=T, E=E, top_k=top_k, n_group=n_group, topk_group=topk_group, dtype=_DTYPE[logits.dtype],
-        bias_dtype=_DTYPE[bias.dtype] if bias is not None else 0, score=_choice(_SCORE, score, "score"),
-        group_score=_choice(_GROUP_SCORE, group_score, "group_score"), renormalize=1 if renormalize else 0, scale=scale), logits.device)
+    ids = logits.new_empty((T, top_k), dtype=torch.int32)
+    w = logits.new_empty((T, top_k), dtype=torch.float32)
+    _launch(_lib.ROUTE, logits.device, logits.data_ptr(), ld, _p(bias), ids.data_ptr(), w.data_ptr(), T, E, top_k, n_group, topk_group,
+            _DTYPE[logits.dtype], 0 if bias is None else _DTYPE[bias.dtype], _choice(_SCORE, score, "score"),
+            _choice(_GROUP_SCORE, group_score, "group_score"), 1 if renormalize else 0, scale)
     return ids, w
 
 
@@ -275,19 +282,15 @@ def route_backward(grad_weights: torch.Tensor, logits: torch.Tensor, ids: torch.
                    renormalize: bool = True, scale: float = 1.0):
     """Gradient of :func:`route`'s weights with respect to the logits, the choice held fixed: [T, E] of the logits' type."""
     _check_float(logits, "logits")
-    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
-        raise ValueError("logits must be [T, E] with unit column stride")
-    T, E = logits.shape
+    T, E, ld = _rows(logits, "logits", 1)
     if ids.dim() != 2:
         raise ValueError("ids must be [T, top_k]")
     top_k = ids.shape[1]
     _check_like(ids, "ids", (T, top_k), torch.int32, logits.device)
     _check_like(grad_weights, "grad_weights", (T, top_k), torch.float32, logits.device)
-    out = torch.empty((T, E), dtype=logits.dtype, device=logits.device)
-    _launch("moe_route_backward", _lib.RouteGradArgs(
-        grad_weights=_p(grad_weights), logits=_p(logits), stride=max(logits.stride(0), E) if T < 2 else logits.stride(0), ids=_p(ids),
-        dlogits=_p(out), T=T, E=E, top_k=top_k, dtype=_DTYPE[logits.dtype], score=_choice(_SCORE, score, "score"),
-        renormalize=1 if renormalize else 0, scale=scale), logits.device)
+    out = torch.empty_like(logits, memory_format=torch.contiguous_format)
+    _launch(_lib.ROUTE_GRAD, logits.device, grad_weights.data_ptr(), logits.data_ptr(), ld, ids.data_ptr(), out.data_ptr(), T, E, top_k,
+            _DTYPE[logits.dtype], _choice(_SCORE, score, "score"), 1 if renormalize else 0, scale)
     return out
 
 
@@ -320,7 +323,7 @@ def quant_fp4(x: torch.Tensor, fmt: str = "nvfp4", global_scale: torch.Tensor | 
         G, src_rows, cols = x.shape
         ld, lead = cols, (G,)
     else:
-        ld, (src_rows, cols), G, lead = _row_stride(x, "x"), x.shape, 1, ()
+        (src_rows, cols, ld), G, lead = _rows(x, "x"), 1, ()
     if act is not None and cols % 2:
         raise ValueError("with act='silu_mul' x must be [rows, 2K]")
     K = cols // 2 if act is not None else cols
@@ -348,14 +351,12 @@ def quant_fp4(x: torch.Tensor, fmt: str = "nvfp4", global_scale: torch.Tensor | 
         _check_like(q, "out[0]", q_shape, torch.uint8, x.device)
         _check_like(s, "out[1]", s_shape, torch.uint8, x.device)
     else:
-        make = torch.empty if src_pair is None else torch.zeros
-        q, s = make(q_shape, dtype=torch.uint8, device=x.device), make(s_shape, dtype=torch.uint8, device=x.device)
+        make = x.new_empty if src_pair is None else x.new_zeros
+        q, s = make(q_shape, dtype=torch.uint8), make(s_shape, dtype=torch.uint8)
     if G == 0 or rows == 0:
         return q, s
-    _launch("moe_quant_fp4", _lib.Fp4QuantArgs(
-        x=_p(x), x_stride=ld, factor=_p(global_scale), factor_stride=gs, src_pair=_p(src_pair), q=_p(q), scales=_p(s), groups=G,
-        rows=rows, src_rows=src_rows, K=K, top_k=top_k, dtype=_DTYPE[x.dtype], format=_FP4_FORMAT[fmt],
-        silu_mul=1 if act is not None else 0, gate_first=1 if gate_first else 0), x.device)
+    _launch(_lib.FP4_QUANT, x.device, x.data_ptr(), ld, _p(global_scale), gs, _p(src_pair), q.data_ptr(), s.data_ptr(), G, rows, src_rows, K,
+            top_k, _DTYPE[x.dtype], _FP4_FORMAT[fmt], 1 if act is not None else 0, 1 if gate_first else 0)
     return q, s
 
 
@@ -363,7 +364,6 @@ def unpack_fp4(q: torch.Tensor):
     """Packed codes uint8 [.., K/2] -> their values as e4m3 [.., K] (every e2m1 value is one)."""
     if q.dtype != torch.uint8 or not q.is_cuda or not q.is_contiguous() or q.dim() == 0 or q.shape[-1] % 8:
         raise ValueError("q must be a contiguous uint8 CUDA tensor whose last dimension is a multiple of 8")
-    out = torch.empty((*q.shape[:-1], 2 * q.shape[-1]), dtype=torch.float8_e4m3fn, device=q.device)
-    with torch.cuda.device(q.device):
-        _lib.check(_lib.lib().moe_unpack_fp4(_vp(q.data_ptr()), _vp(out.data_ptr()), _i64(q.numel()), _stream(q)))
+    out = q.new_empty((*q.shape[:-1], 2 * q.shape[-1]), dtype=torch.float8_e4m3fn)
+    _launch(_lib.UNPACK_FP4, q.device, q.data_ptr(), out.data_ptr(), q.numel())
     return out
