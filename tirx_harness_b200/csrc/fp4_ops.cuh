@@ -32,24 +32,39 @@ struct Fp4QuantParams {
     int k_blocks;                               // 256-column pieces of K
 };
 
-// eight values -> eight codes, the first in the lowest four bits
+// eight values -> eight codes, the first in the lowest four bits.  The bytes are put together by multiplications, which run
+// beside the conversions' pipe.
 __device__ __forceinline__ uint32_t pack8_e2m1(const f32x2 (&v)[4]) {
     uint32_t r = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        r |= (uint32_t)__nv_cvt_float2_to_fp4x2(make_float2(lo2(v[i]), hi2(v[i])), __NV_E2M1, cudaRoundNearest) << (8 * i);
+    for (int i = 3; i >= 0; --i) {
+        const uint32_t b = __nv_cvt_float2_to_fp4x2(make_float2(lo2(v[i]), hi2(v[i])), __NV_E2M1, cudaRoundNearest);
+        if (i == 3) r = b;
+        else asm("mad.lo.u32 %0, %1, 256, %2;" : "=r"(r) : "r"(r), "r"(b));
+    }
     return r;
 }
 
-// The largest magnitude of 16 values.  As unsigned numbers the magnitudes of a 16-bit type are in order, with infinity and
-// NaN above the others, and two of them are compared at a time.
+// The larger magnitudes of two pairs of 16-bit values; a NaN stays one.
+template <typename T> __device__ __forceinline__ uint32_t amax2_nan(uint32_t m, uint32_t u);
+template <> __device__ __forceinline__ uint32_t amax2_nan<__nv_bfloat16>(uint32_t m, uint32_t u) {
+    uint32_t r;
+    asm("{\n\t.reg .b32 t;\n\tabs.bf16x2 t, %2;\n\tmax.NaN.bf16x2 %0, %1, t;\n\t}" : "=r"(r) : "r"(m), "r"(u));
+    return r;
+}
+template <> __device__ __forceinline__ uint32_t amax2_nan<__half>(uint32_t m, uint32_t u) {
+    uint32_t r;
+    asm("{\n\t.reg .b32 t;\n\tabs.f16x2 t, %2;\n\tmax.NaN.f16x2 %0, %1, t;\n\t}" : "=r"(r) : "r"(m), "r"(u));
+    return r;
+}
+// The largest magnitude of 16 values.
 template <typename T> __device__ __forceinline__ float largest16(const Raw8<T>& a, const Raw8<T>& b) {
     uint32_t m = 0;
     const uint32_t u[8] = {a.w[0].x, a.w[0].y, a.w[0].z, a.w[0].w, b.w[0].x, b.w[0].y, b.w[0].z, b.w[0].w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = __vmaxu2(m, u[i] & 0x7FFF7FFFu);
-    m = max(m & 0xFFFFu, m >> 16);
-    return lo2(Fmt<T>::up(m));
+    for (int i = 0; i < 8; ++i) m = amax2_nan<T>(m, u[i]);
+    const f32x2 f = Fmt<T>::up(m);
+    return amax_nan(lo2(f), hi2(f));
 }
 template <> __device__ __forceinline__ float largest16<float>(const Raw8<float>& a, const Raw8<float>& b) {
     uint32_t m = 0;
@@ -75,8 +90,11 @@ constexpr int FP4_QUANT_THREADS = 256, FP4_QUANT_ROWS = 64;
 // NV: nvfp4, else mxfp4.  SILU: x holds gate and up, K columns each.
 // Block: 64 rows x 256 columns.  A thread takes 16 columns of a row at a time (a block of nvfp4, half a block of mxfp4) and
 // four such rows in all: of 16-bit inputs all four are loaded before the first is used, of the others two at a time.
+// Blocks per SM as measured (16384 x 7168 nvfp4: 3, 4, 5 blocks 66, 61, 66 us; mxfp4: 4, 5, 6 blocks 48, 46, 61 us; SiLU*mul of
+// 16384 x 2048: 2, 3, 4 blocks 42, 35, 39 us).  mxfp4 runs at memory's speed; nvfp4 has a division more per value and is
+// bound by the instructions around its conversions.
 template <typename T, bool NV, bool SILU>
-__global__ void __launch_bounds__(FP4_QUANT_THREADS) quant_fp4_kernel(const Fp4QuantParams p) {
+__global__ void __launch_bounds__(FP4_QUANT_THREADS, sizeof(T) == 2 ? (SILU ? 3 : (NV ? 4 : 5)) : 2) quant_fp4_kernel(const Fp4QuantParams p) {
     constexpr int WORDS = NV ? 4 : 2;           // scale tiles of 256 columns
     constexpr int STEP = FP4_QUANT_THREADS / 16, ROWS = FP4_QUANT_ROWS / STEP, BATCH = sizeof(T) == 2 && !SILU ? ROWS : ROWS / 2;
     __shared__ uint32_t tile[WORDS][FP4_QUANT_ROWS];
@@ -176,18 +194,24 @@ __global__ void __launch_bounds__(FP4_QUANT_THREADS) quant_fp4_kernel(const Fp4Q
     }
 }
 
-// Packed codes -> e4m3 values, 16 per thread.
-__global__ void __launch_bounds__(256) unpack_fp4_kernel(const uint2* __restrict__ q, uint4* __restrict__ out, long long n) {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n) return;
-    const uint2 w = __ldcs(q + i);
+// Packed codes -> e4m3 values, 8 bytes to 16; a thread loads four of them before it stores the first.
+constexpr int FP4_UNPACK_THREADS = 256, FP4_UNPACK_EACH = 4;
+__global__ void __launch_bounds__(FP4_UNPACK_THREADS) unpack_fp4_kernel(const uint2* __restrict__ q, uint4* __restrict__ out, long long n) {
     // magnitudes 0 .5 1 1.5 | 2 3 4 6 as e4m3 bytes; a code's low three bits pick one, its fourth is the sign
     auto four = [](uint32_t c) {
         const uint32_t mag = __byte_perm(0x3C383000u, 0x4C484440u, c & 0x7777u);
         const uint32_t sign = ((c & 0x8u) << 4) | ((c & 0x80u) << 8) | ((c & 0x800u) << 12) | ((c & 0x8000u) << 16);
         return mag | sign;
     };
-    __stcs(out + i, make_uint4(four(w.x & 0xFFFFu), four(w.x >> 16), four(w.y & 0xFFFFu), four(w.y >> 16)));
+    const long long i0 = (long long)blockIdx.x * (FP4_UNPACK_THREADS * FP4_UNPACK_EACH) + threadIdx.x;
+    uint2 w[FP4_UNPACK_EACH];
+#pragma unroll
+    for (int k = 0; k < FP4_UNPACK_EACH; ++k)
+        if (i0 + k * FP4_UNPACK_THREADS < n) w[k] = __ldcs(q + i0 + k * FP4_UNPACK_THREADS);
+#pragma unroll
+    for (int k = 0; k < FP4_UNPACK_EACH; ++k)
+        if (i0 + k * FP4_UNPACK_THREADS < n)
+            __stcs(out + i0 + k * FP4_UNPACK_THREADS, make_uint4(four(w[k].x & 0xFFFFu), four(w[k].x >> 16), four(w[k].y & 0xFFFFu), four(w[k].y >> 16)));
 }
 
 }  // namespace b200

@@ -398,9 +398,10 @@ int moe_unpack_fp4(const void* q, void* out_e4m3, int64_t n_bytes, void* stream)
     if (n_bytes < 0 || n_bytes % 8) return fail(MOE_ERR_INVALID, "n_bytes must be a non-negative multiple of 8");
     if (n_bytes == 0) return MOE_OK;
     if (!q || !out_e4m3 || !aligned16(q) || !aligned16(out_e4m3)) return fail(MOE_ERR_INVALID, "q and out must be non-NULL and 16-byte aligned");
-    const long long n = n_bytes / 8, blocks = (n + 255) / 256;
+    constexpr int each = FP4_UNPACK_THREADS * FP4_UNPACK_EACH;
+    const long long n = n_bytes / 8, blocks = (n + each - 1) / each;
     if (blocks > 0x7FFFFFFFll) return fail(MOE_ERR_INVALID, "n_bytes exceeds what one call covers");
-    unpack_fp4_kernel<<<(unsigned)blocks, 256, 0, static_cast<cudaStream_t>(stream)>>>(static_cast<const uint2*>(q), static_cast<uint4*>(out_e4m3), n);
+    unpack_fp4_kernel<<<(unsigned)blocks, FP4_UNPACK_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(static_cast<const uint2*>(q), static_cast<uint4*>(out_e4m3), n);
     CUDA_TRY(cudaGetLastError());
     return MOE_OK;
 }
