@@ -111,38 +111,43 @@ __device__ __forceinline__ int build_pair_list(const GGFp4Params& p, int* list, 
         for (int j = 0; j < 4; ++j) if (v[j] > g) m = min(m, v[j]);
         return __reduce_min_sync(0xffffffffu, m);
     };
-#pragma unroll 2
-    for (int b = warp; b < nb; b += warps) {
-        int v[4];
-        load(b, v);
-        int g = after(v, -1), n = 0;
-        const int first = g;
-        while (g != INT_MAX) { ++n; g = after(v, g); }
-        if (lane == 0) { count[b] = n; lowest[b] = first; }
+    constexpr int AHEAD = 8;                         // blocks under way per warp
+    for (int b0 = warp * AHEAD; b0 < nb; b0 += warps * AHEAD) {
+        int v[AHEAD][4];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) load(b0 + k, v[k]);
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            if (b0 + k >= nb) break;
+            const int first = after(v[k], -1);
+            int most = -1, n = first != INT_MAX;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) if (v[k][j] != INT_MAX) most = max(most, v[k][j]);
+            most = __reduce_max_sync(0xffffffffu, most);
+            if (most != first)
+                for (int g = first; g < most; ++n) g = after(v[k], g);
+            if (lane == 0) { count[b0 + k] = n; lowest[b0 + k] = first; }
+        }
     }
     __syncthreads();
     int total = 0;                                   // the same in every warp
     for (int base = 0; base < nb; base += 32) {
-        const int n = base + lane < nb ? count[base + lane] : 0;
+        const int b = base + lane, n = b < nb ? count[b] : 0;
         int incl = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int u = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += u;
         }
-        // warp w writes the entries of the blocks w, w + warps, ..: a block with one group at once
-        for (unsigned todo = __ballot_sync(0xffffffffu, base + lane < nb && n > 0 && (base + lane) % warps == warp); todo; todo &= todo - 1) {
-            const int i = __ffs(todo) - 1, b = base + i;
-            int at = total + __shfl_sync(0xffffffffu, incl - n, i);
-            const int m = __shfl_sync(0xffffffffu, n, i);
-            if (at + m > PAIR_LIST_CAP) continue;
-            if (m == 1) {
-                if (lane == 0) entry[at] = b | lowest[b] << PAIR_LIST_BLOCK_BITS;
-            } else {
-                int v[4];
-                load(b, v);
-                for (int g = after(v, -1); g != INT_MAX; g = after(v, g), ++at)
-                    if (lane == 0) entry[at] = b | g << PAIR_LIST_BLOCK_BITS;
+        const int at = total + incl - n;
+        if ((base >> 5) % warps == warp) {
+            if (n == 1 && at < PAIR_LIST_CAP) entry[at] = b | lowest[b] << PAIR_LIST_BLOCK_BITS;
+            for (unsigned todo = __ballot_sync(0xffffffffu, n > 1 && at + n <= PAIR_LIST_CAP); todo; todo &= todo - 1) {
+                const int i = __ffs(todo) - 1;
+                int to = __shfl_sync(0xffffffffu, at, i), v[4];
+                load(base + i, v);
+                for (int g = after(v, -1); g != INT_MAX; g = after(v, g), ++to)
+                    if (lane == 0) entry[to] = (base + i) | g << PAIR_LIST_BLOCK_BITS;
             }
         }
         total += __shfl_sync(0xffffffffu, incl, 31);
@@ -445,32 +450,36 @@ gg_fp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
 }
 
 // ------------------------------------------------------------------ few rows per group
-// gg_fp4_few_kernel: the weights' rows are the MMA's M (128 per tile), the group's rows its N (at most NT = 32 or 128), so a
-// tile streams 128 rows of B over all of K and multiplies little in vain.  Bound by reading the weights from HBM: two
-// blocks per SM (NT = 32) keep four 16 KB stages each under way.  Two accumulators: a tile is stored while the next one is
-// multiplied.  Blocks come in clusters of CLUSTER.  Where there are more tiles than clusters, every block takes tiles of its
-// own; with fewer, the blocks of a cluster take a part of K each and add their sums up, always in the same order, through
-// each other's shared memory.  Clusters of two: 74 of them fit, clusters of four only on 132 of the 148 SMs, which
-// costs 32 groups of 8 rows (4096 x 7168) 104 us instead of 82.  Clusters of four where no more than 32 tiles can come:
-// one row, 4096 x 4096, 6.0 us instead of 7.4.
+// gg_fp4_few_kernel: the weights' rows are the MMA's M (128 per tile), up to NT = 32 or 128 rows of a group its N, so a tile
+// streams 128 rows of B over all of K and multiplies little in vain.  Bound by reading the weights from HBM: two blocks per
+// SM (NT = 32) keep four 16 KB stages each under way (8 rows in 32 groups, 4096 x 7168: 82 us, 6.4 TB/s; one row in 8 groups:
+// 23 us).  Two accumulators: a tile is stored while the next one is multiplied.  Blocks come in clusters of CLUSTER.  Where
+// there are more tiles than clusters, or K is short, every block takes tiles of its own; else the blocks of a cluster take
+// a part of K each and add their sums up, always in the same order, through each other's shared memory (one row, 4096 x
+// 7168: 7.6 us instead of 11.2).  Clusters of two, of which 74 fit; clusters of four fit on 132 of the 148 SMs only, which
+// costs 32 groups of 8 rows 104 us instead of 82, and serve calls that cannot have more than 32 tiles.
 namespace ff {
 constexpr int BKB = 128, THREADS = 256, ACCS = 2;
 constexpr int FOUR_MAX_TILES = 32;
+constexpr int LIST_CAP = 1024;               // (group, chunk of rows) entries: the host sees to it that there are no more,
+constexpr int MAX_ROWS = 1024;               // nor more rows in the contiguous layout
 template <bool NV, int NT> struct Cfg {
     static constexpr int SF_CHUNK = NV ? 2048 : 1024;
     static constexpr int W_BYTES = 128 * BKB, X_BYTES = NT * BKB;
     static constexpr int STAGE = W_BYTES + X_BYTES + 2 * SF_CHUNK;
     static constexpr int STAGES = NT == 32 ? 4 : 5;
     static constexpr int BLOCKS_PER_SM = NT == 32 ? 2 : 1;
+    // a stage of K takes 0.25 us, adding the blocks' sums up 1.7 us (NT = 32) or 2.5 us: where K is shorter it is not shared
+    static constexpr int SPLIT_MIN_KB = NT == 32 ? 16 : 24;
     static constexpr int SF_COLS = NV ? 16 : 8;                  // scale columns of one operand and stage
     static constexpr int COLS = ACCS * NT + STAGES * 2 * SF_COLS, TMEM_COLS = COLS > 256 ? 512 : (COLS > 128 ? 256 : 128);
     static constexpr int OFF_X = STAGES * W_BYTES;
     static constexpr int OFF_SF = OFF_X + STAGES * X_BYTES;
     static constexpr int OFF_BARS = OFF_SF + STAGES * 2 * SF_CHUNK;
     static constexpr int OFF_LIST = OFF_BARS + 256;
-    static constexpr int SMEM_BYTES = OFF_LIST + gg::MAX_MASKED_GROUPS * 4 + 1024;
+    static constexpr int SMEM_BYTES = OFF_LIST + LIST_CAP * 4 + 1024;
     static_assert(COLS <= 512 && BLOCKS_PER_SM * TMEM_COLS <= 512, "accumulators and scales must fit TMEM");
-    static_assert(STAGES * STAGE >= NT * 128 * 4, "the ring's memory holds the sums of a cluster's blocks for one block's columns");
+    static_assert(STAGES * STAGE >= NT / 8 * 128 * 12 * 4, "the ring's memory holds the sums of a cluster's blocks for one block's rows");
 };
 }  // namespace ff
 
@@ -491,11 +500,22 @@ __device__ __forceinline__ void umma_fp4(uint32_t tmem_d, uint64_t adesc, uint64
             ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(tmem_sfa), "r"(tmem_sfb) : "memory");
 }
 
-// 32 rows of one column of d: row j, where bit j of `rows` is set, at d + j * ldd
-template <typename T>
-__device__ __forceinline__ void few_store(T* d, long long ldd, unsigned rows, const uint32_t (&v)[32], float alpha) {
+// S accumulator columns (8 or 16), i.e. rows of d, of this warp's 32 lanes, i.e. columns of d
+template <int S> __device__ __forceinline__ void few_load(uint32_t taddr, uint32_t (&v)[S]) {
+    static_assert(S == 8 || S == 16, "");
+    if constexpr (S == 8) {
+        tmem_ld_32x32b_x8(taddr, v);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7])::"memory");
+    } else {
+        tmem_ld_32x32b_x16(taddr, v);
+        tmem_ld_wait(v);
+    }
+}
+// S rows of one column of d: row j, where bit j of `rows` is set, at d + j * ldd
+template <typename T, int S>
+__device__ __forceinline__ void few_store(T* d, long long ldd, unsigned rows, const uint32_t (&v)[S], float alpha) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j, d += ldd)
+    for (int j = 0; j < S; ++j, d += ldd)
         if ((rows >> j) & 1u) *d = from_f32<T>(__uint_as_float(v[j]) * alpha);
 }
 
@@ -511,7 +531,7 @@ gg_fp4_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BARS);          // full[S], empty[S], tmem_full[2], tmem_empty[2]
     uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 4);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_base_slot + 1);
-    int* list = reinterpret_cast<int*>(smem + C::OFF_LIST);                    // the groups that have rows
+    int* list = reinterpret_cast<int*>(smem + C::OFF_LIST);                    // group | chunk of NT rows << 20, where it has rows
     volatile int* list_len = reinterpret_cast<volatile int*>(tmem_base_slot + 2);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t full_bar = smem_u32(bars), empty_bar = smem_u32(bars + STAGES);
@@ -536,38 +556,49 @@ gg_fp4_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
         tmem_alloc(smem_u32(tmem_base_slot), C::TMEM_COLS);
         tmem_relinquish();
     }
+    int* groups = reinterpret_cast<int*>(smem);            // contiguous layout: the rows' groups, in the ring's memory for now
+    if (!p.masked) {
+        for (int r = threadIdx.x; r < p.M; r += THREADS) groups[r] = r < rows_end ? __ldg(p.layout + r) : -1;
+        __syncthreads();
+    }
     if (warp == 2) {
         int n = 0;
         if (p.masked) {
             for (int base = 0; base < p.G; base += 32) {
-                const bool has = base + lane < p.G && __ldg(p.layout + base + lane) > 0;
-                const unsigned b = __ballot_sync(0xffffffffu, has);
-                if (has) list[n + __popc(b & ((1u << lane) - 1u))] = base + lane;
-                n += __popc(b);
+                const int g = base + lane, rows = g < p.G ? min(p.M, max(0, __ldg(p.layout + g))) : 0, chunks = (rows + NT - 1) / NT;
+                int incl = chunks;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int v = __shfl_up_sync(0xffffffffu, incl, o);
+                    if (lane >= o) incl += v;
+                }
+                for (int c = 0; c < chunks; ++c) list[n + incl - chunks + c] = g | c << 20;
+                n += __shfl_sync(0xffffffffu, incl, 31);
             }
         } else {
-            // the distinct groups of the (at most NT) rows, ascending
-            int vals[NT / 32];
+            for (int row0 = 0; row0 < p.M; row0 += NT) {
+                // the distinct groups of the chunk's rows, ascending
+                int vals[NT / 32];
 #pragma unroll
-            for (int j = 0; j < NT / 32; ++j) {
-                const int r = lane + 32 * j;
-                vals[j] = r < rows_end ? __ldg(p.layout + r) : -1;
-            }
-            int after = -1;
-            while (true) {
-                int best = INT_MAX;
+                for (int j = 0; j < NT / 32; ++j) {
+                    const int r = row0 + lane + 32 * j;
+                    vals[j] = r < p.M ? groups[r] : -1;
+                }
+                for (int after = -1;; ++n) {
+                    int best = INT_MAX;
 #pragma unroll
-                for (int j = 0; j < NT / 32; ++j)
-                    if (vals[j] > after && vals[j] < p.G && vals[j] < best) best = vals[j];
-                best = __reduce_min_sync(0xffffffffu, best);
-                if (best == INT_MAX) break;
-                if (lane == 0) list[n] = best;
-                ++n;
-                after = best;
+                    for (int j = 0; j < NT / 32; ++j)
+                        if (vals[j] > after && vals[j] < p.G && vals[j] < best) best = vals[j];
+                    best = __reduce_min_sync(0xffffffffu, best);
+                    if (best == INT_MAX) break;
+                    if (lane == 0) list[n] = best | (row0 / NT) << 20;
+                    after = best;
+                }
             }
         }
         if (lane == 0) *list_len = n;
     }
+    fence_proxy_async_smem();                     // bulk copies write the ring from here on
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -576,7 +607,7 @@ gg_fp4_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
     const int tiles = *list_len * n_tiles, clusters = gridDim.x / CLUSTER;
     const int rank = (int)cluster_ctarank(), cluster = blockIdx.x / CLUSTER;
     // few tiles: one per cluster, a part of K per block; else one after the other per block, spread over the clusters first
-    const bool split = tiles <= clusters;
+    const bool split = tiles <= clusters && KB >= C::SPLIT_MIN_KB;
     const int first = split ? cluster : rank * clusters + cluster, step = gridDim.x;
     const int kb0 = split ? KB * rank / CLUSTER : 0, kb1 = split ? KB * (rank + 1) / CLUSTER : KB;
 
@@ -585,10 +616,11 @@ gg_fp4_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
         uint32_t stage = 0, phase = 0;
         bool ok = true;
         for (int t = first; ok && t < tiles; t += step) {
-            const int g = list[t / n_tiles], nt = t % n_tiles;
-            const int w_row = g * p.N + nt * 128, x_row = p.masked ? g * p.M : 0;
+            const int e = list[t / n_tiles], g = e & 0xFFFFF, chunk = e >> 20, nt = t % n_tiles;
+            const int w_row = g * p.N + nt * 128, x_row = (p.masked ? g * p.M : 0) + chunk * NT;
             const uint8_t* sfw = p.sfb + ((long long)g * p.b_tiles + nt) * KB * C::SF_CHUNK;
-            const uint8_t* sfx = p.sfa + (p.masked ? (long long)g * p.a_tiles : 0) * KB * C::SF_CHUNK;
+            // (NT = 32 has one chunk)
+            const uint8_t* sfx = p.sfa + ((p.masked ? (long long)g * p.a_tiles : 0) + chunk) * KB * C::SF_CHUNK;
             for (int kb = kb0; kb < kb1; ++kb) {
                 ok = mbar_wait_warp(empty_bar + 8 * stage, phase ^ 1, abort_flag, status, STATUS_TIMEOUT_SMEM_EMPTY);
                 if (!ok) break;
@@ -614,7 +646,7 @@ gg_fp4_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
         const uint64_t wdesc0 = make_smem_desc_sw128(smem_u32(smem)), xdesc0 = make_smem_desc_sw128(smem_u32(smem + C::OFF_X));
         const uint64_t sdesc0 = make_sf_desc(smem_u32(smem + C::OFF_SF));
         const uint32_t idesc = make_idesc_fp4<NV>(128, NT, 0);
-        for (int t = first; ok && t < tiles && kb0 < kb1; t += step) {
+        for (int t = first; ok && t < tiles; t += step) {
             ok = mbar_wait_warp(tempty_bar + 8 * acc, acc_phase ^ 1, abort_flag, status, STATUS_TIMEOUT_TMEM_EMPTY);
             if (!ok) break;
             tc_fence_after();
@@ -648,85 +680,101 @@ gg_fp4_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
     }
     // ---------------------------------------------------- epilogue: thread = column of d, register = row
     const int ew = warp - 4;                       // TMEM lane quarter (warp % 4)
-    // which of the 32 rows from row0 on belong to group g
+    // Rows are taken S at a time: the code is short, which is what a call of one tile waits for (unrolled over 32 rows, the
+    // instruction fetches alone took 2 us), and a call with few rows runs through it once.
+    constexpr int S = NT == 32 ? 8 : 16;
+    // which of the S rows from row0 on belong to group g
     auto rows_of = [&](int g, int row0) -> unsigned {
         if (p.masked) {
             const int left = min(p.M, __ldg(p.layout + g)) - row0;
-            return left >= 32 ? 0xffffffffu : (left > 0 ? (1u << left) - 1u : 0u);
+            return left >= S ? (1u << S) - 1u : (left > 0 ? (1u << left) - 1u : 0u);
         }
-        return __ballot_sync(0xffffffffu, row0 + lane < rows_end && __ldg(p.layout + row0 + lane) == g);
+        return __ballot_sync(0xffffffffu, lane < S && row0 + lane < rows_end && __ldg(p.layout + row0 + lane) == g);
     };
     auto alpha_of = [&](int g) { return p.alpha ? __ldg(p.alpha + g * p.alpha_stride) : 1.0f; };
+    auto put = [&](int g, int row0, int n, unsigned rows, const uint32_t (&v)[S], float alpha) {
+        const long long o = ((p.masked ? (long long)g * p.M : 0) + row0) * p.ldd + n;
+        if (n >= p.N) rows = 0u;
+        if (p.d_f32) few_store(static_cast<float*>(p.d) + o, p.ldd, rows, v, alpha);
+        else few_store(static_cast<__nv_bfloat16*>(p.d) + o, p.ldd, rows, v, alpha);
+    };
     if (warp >= 4 && !split) {
         uint32_t acc = 0, acc_phase = 0;
         for (int t = first; t < tiles; t += step) {
-            const int g = list[t / n_tiles], n = (t % n_tiles) * 128 + ew * 32 + lane;
+            const int e = list[t / n_tiles], g = e & 0xFFFFF, row0 = (e >> 20) * NT, n = (t % n_tiles) * 128 + ew * 32 + lane;
             const float alpha = alpha_of(g);
             if (!mbar_wait_warp(tfull_bar + 8 * acc, acc_phase, abort_flag, status, STATUS_TIMEOUT_TMEM_FULL)) break;
             tc_fence_after();
-            long long o = (p.masked ? (long long)g * p.M * p.ldd : 0) + n;
 #pragma unroll 1
-            for (int w = 0; w < NT; w += 32, o += 32 * p.ldd) {
-                unsigned rows = rows_of(g, w);
-                uint32_t v[32];
-                if (rows != 0u) {
-                    tmem_ld_32x32b_x32(tmem_base + (uint32_t(ew * 32) << 16) + acc * NT + w, v);
-                    tmem_ld_wait(v);
-                }
-                if (w == NT - 32) {            // the accumulator is in registers
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(tempty_bar + 8 * acc);
-                }
-                if (n >= p.N) rows = 0u;
-                if (p.d_f32) few_store(static_cast<float*>(p.d) + o, p.ldd, rows, v, alpha);
-                else few_store(static_cast<__nv_bfloat16*>(p.d) + o, p.ldd, rows, v, alpha);
+            for (int w = 0; w < NT; w += S) {
+                const unsigned rows = rows_of(g, row0 + w);
+                if (rows == 0u) continue;
+                uint32_t v[S];
+                few_load(tmem_base + (uint32_t(ew * 32) << 16) + acc * NT + w, v);
+                put(g, row0 + w, n, rows, v, alpha);
             }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(tempty_bar + 8 * acc);
             if (++acc == ACCS) { acc = 0; acc_phase ^= 1; }
         }
     }
     if (split) {
-        constexpr int F = 128 / CLUSTER;           // columns that a block finishes
+        // S rows at a time belong to the blocks of the cluster in turn, which finish them
         const bool work = first < tiles;
-        const int g = work ? list[first / n_tiles] : 0, n0 = work ? (first % n_tiles) * 128 : 0, c = ew * 32 + lane;
-        if (warp >= 4 && work && kb0 < kb1) mbar_wait_warp(tfull_bar, 0, abort_flag, status, STATUS_TIMEOUT_TMEM_FULL);
+        const int e = work ? list[first / n_tiles] : 0, g = e & 0xFFFFF, row0 = (e >> 20) * NT;
+        const int c = ew * 32 + lane, n = (work ? (first % n_tiles) * 128 : 0) + c;
+        const uint32_t acc = tmem_base + (uint32_t(ew * 32) << 16);
+        if (warp >= 4 && work) mbar_wait_warp(tfull_bar, 0, abort_flag, status, STATUS_TIMEOUT_TMEM_FULL);
         __syncwarp();
-        // every block of the cluster has read all of its stages: their memory takes the sums, [rank][row][F columns]
+        // every block of the cluster has read all of its stages: their memory takes the other blocks' sums of the rows that a
+        // block is to finish, [rank][S rows][column][row] (a thread sends its rows 16 bytes at a time; the distance between
+        // columns keeps the banks apart)
+        constexpr int PITCH = S + 4;
+        auto slot = [&](int from, int w) { return ((from * (NT / CLUSTER / S) + w / S / CLUSTER) * 128 + c) * PITCH; };
         cluster_sync_all();
         if (warp >= 4 && work) {
             tc_fence_after();
-            const uint32_t dst = map_to_cta(smem_u32(smem), c / F) + (rank * NT * F + c % F) * 4;
 #pragma unroll 1
-            for (int w = 0; w < NT; w += 32) {
-                const unsigned rows = rows_of(g, w);
-                if (rows == 0u) continue;
-                uint32_t v[32];
-                tmem_ld_32x32b_x32(tmem_base + (uint32_t(ew * 32) << 16) + w, v);
-                tmem_ld_wait(v);
+            for (int w = 0; w < NT; w += S) {
+                const unsigned rows = rows_of(g, row0 + w);
+                const int owner = w / S % CLUSTER;
+                if (rows == 0u || owner == rank) continue;
+                uint32_t v[S];
+                few_load(acc + w, v);
+                const uint32_t dst = map_to_cta(smem_u32(smem), owner) + slot(rank, w) * 4;
 #pragma unroll
-                for (int j = 0; j < 32; ++j)
-                    if ((rows >> j) & 1u)
-                        asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(dst + (w + j) * F * 4), "r"(kb0 < kb1 ? v[j] : 0u) : "memory");
+                for (int j = 0; j < S; j += 4)
+                    asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};"
+                                 ::"r"(dst + j * 4), "r"(v[j]), "r"(v[j + 1]), "r"(v[j + 2]), "r"(v[j + 3]) : "memory");
             }
         }
         __syncwarp();
         cluster_sync_all();
         if (warp >= 4 && work) {
             const float alpha = alpha_of(g);
-            const int n = n0 + rank * F + c % F;
-            const float* part = reinterpret_cast<const float*>(smem) + c % F;
 #pragma unroll 1
-            for (int w = 0; w < NT; w += 32) {
-                const unsigned rows = rows_of(g, w);
-                for (int j = c / F; j < 32; j += CLUSTER)
-                    if (((rows >> j) & 1u) && n < p.N) {
-                        float v = part[(w + j) * F];
+            for (int w = rank * S; w < NT; w += CLUSTER * S) {
+                const unsigned rows = rows_of(g, row0 + w);
+                if (rows == 0u) continue;
+                uint32_t v[S];
+                few_load(acc + w, v);
+                float sum[S];
 #pragma unroll
-                        for (int r = 1; r < CLUSTER; ++r) v += part[(r * NT + w + j) * F];
-                        const long long o = ((p.masked ? (long long)g * p.M : 0) + w + j) * p.ldd + n;
-                        if (p.d_f32) static_cast<float*>(p.d)[o] = v * alpha;
-                        else static_cast<__nv_bfloat16*>(p.d)[o] = __float2bfloat16_rn(v * alpha);
+                for (int j = 0; j < S; ++j) sum[j] = 0.0f;
+#pragma unroll 1
+                for (int r = 0; r < CLUSTER; ++r) {        // in the order of the ranks
+                    const float4* part = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem) + slot(r, w));
+#pragma unroll
+                    for (int j = 0; j < S; j += 4) {
+                        float4 x = make_float4(__uint_as_float(v[j]), __uint_as_float(v[j + 1]), __uint_as_float(v[j + 2]), __uint_as_float(v[j + 3]));
+                        if (r != rank) x = part[j / 4];
+                        sum[j] += x.x; sum[j + 1] += x.y; sum[j + 2] += x.z; sum[j + 3] += x.w;
                     }
+                }
+#pragma unroll
+                for (int j = 0; j < S; ++j) v[j] = __float_as_uint(sum[j]);
+                put(g, row0 + w, n, rows, v, alpha);
             }
         }
     }

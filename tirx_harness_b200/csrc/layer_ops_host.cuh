@@ -183,7 +183,8 @@ int launch_fp4_pair(const GGFp4Params& p, long long rows_total, DeviceInfo* di, 
     GGParams sp = {};
     sp.layout = p.layout; sp.rows_used = p.rows_used; sp.G = p.G; sp.M = p.M; sp.N = p.N;
     sp.num_n_blocks = (p.N + TN - 1) / TN;
-    const long long blocks = MASKED ? (long long)p.G * ((p.M + 255) / 256) : (p.M + 255) / 256;
+    // row blocks that sorted rows can fill (more tiles than this only make the pairs take more than one each)
+    const long long blocks = MASKED ? (long long)p.G * ((p.M + 255) / 256) : (p.M + 255) / 256 + (p.G < p.M ? p.G : p.M) - 1;
     const long long tiles = blocks * sp.num_n_blocks;
     const int pairs = (int)(tiles < di->max_pairs ? tiles : di->max_pairs);
     static std::atomic<uint64_t> done{0};
@@ -195,6 +196,14 @@ int launch_fp4_pair(const GGFp4Params& p, long long rows_total, DeviceInfo* di, 
 template <bool NV, int TN>
 int launch_fp4_pair_layout(const GGFp4Params& p, long long rows_total, DeviceInfo* di, cudaStream_t st) {
     return p.masked ? launch_fp4_pair<NV, true, TN>(p, rows_total, di, st) : launch_fp4_pair<NV, false, TN>(p, rows_total, di, st);
+}
+
+// the most (group, chunk of NT rows) that can have rows
+long long fp4_few_entries(const GGFp4Params& p, int NT) {
+    const long long chunks = (p.M + NT - 1) / NT;
+    if (p.masked) return p.G * chunks;
+    // a chunk has at most NT groups; sorted rows change groups G - 1 times at most, but they need not be sorted
+    return chunks * (p.G < NT ? p.G : NT) < p.M ? chunks * (p.G < NT ? p.G : NT) : p.M;
 }
 
 template <bool NV, int NT, int CLUSTER>
@@ -217,7 +226,7 @@ int launch_fp4_few_clusters(const GGFp4Params& p, long long rows_total, long lon
 template <bool NV, int NT>
 int launch_fp4_few(const GGFp4Params& p, long long rows_total, DeviceInfo* di, cudaStream_t st) {
     // the most tiles that can come: the groups with rows are known on the device only
-    const long long tiles = (long long)(p.masked || p.G < p.M ? p.G : p.M) * ((p.N + 127) / 128);
+    const long long tiles = fp4_few_entries(p, NT) * ((p.N + 127) / 128);
     return tiles <= ff::FOUR_MAX_TILES ? launch_fp4_few_clusters<NV, NT, 4>(p, rows_total, tiles, di, st)
                                        : launch_fp4_few_clusters<NV, NT, 2>(p, rows_total, tiles, di, st);
 }
@@ -255,8 +264,14 @@ int launch_gg_fp4(const moe_gg_fp4_args* a, bool masked, void* stream) {
     p.a_tiles = (a->M + 127) / 128; p.b_tiles = (a->N + 127) / 128;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool nv = a->format == MOE_FP4_NV;
-    if (a->M <= 32) return nv ? launch_fp4_few<true, 32>(p, rows_total, di, st) : launch_fp4_few<false, 32>(p, rows_total, di, st);
-    if (a->M <= 128) return nv ? launch_fp4_few<true, 128>(p, rows_total, di, st) : launch_fp4_few<false, 128>(p, rows_total, di, st);
+    if (a->M <= 32 && a->G <= (1 << 20)) return nv ? launch_fp4_few<true, 32>(p, rows_total, di, st) : launch_fp4_few<false, 32>(p, rows_total, di, st);
+    // Tiles of 128 x 128 and one block each where one round of them covers the matrix: pairs of blocks on 256 x 256 would
+    // leave most SMs idle (8 groups of 200 rows, 1024 x 1024: 7.3 us against 8.8; one of 256, 4096 x 7168: 13.1 against 15.3),
+    // with more tiles they read less (one of 1024 rows, 4096 x 7168: 26 us against 19).
+    const long long row_chunks = (a->M + 127) / 128 * (masked ? (long long)a->G : 1);
+    const bool one_round = row_chunks * ((a->N + 127) / 128) <= di->num_sms && fp4_few_entries(p, 128) <= ff::LIST_CAP &&
+                           (masked || a->M <= ff::MAX_ROWS) && a->G <= (1 << 20);
+    if ((a->M <= 128 && a->G <= (1 << 20)) || one_round) return nv ? launch_fp4_few<true, 128>(p, rows_total, di, st) : launch_fp4_few<false, 128>(p, rows_total, di, st);
     return nv ? launch_fp4_pair_layout<true, 256>(p, rows_total, di, st) : launch_fp4_pair_layout<false, 256>(p, rows_total, di, st);
 }
 
