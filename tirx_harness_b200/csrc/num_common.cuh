@@ -85,6 +85,12 @@ template <typename T> __device__ __forceinline__ void store8(T* p, const Raw8<T>
     for (int i = 0; i < (int)(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(p)[i] = r.w[i];
 }
 
+// the same for data that is not wanted in the L2 cache any longer
+template <typename T> __device__ __forceinline__ void store8_streaming(T* p, const Raw8<T>& r) {
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(T) / 2); ++i) __stcs(reinterpret_cast<uint4*>(p) + i, r.w[i]);
+}
+
 // the larger magnitude; a NaN stays one
 __device__ __forceinline__ float amax_nan(float a, float b) {
     float r;
@@ -96,6 +102,13 @@ __device__ __forceinline__ float amax_nan(float a, float b) {
 __device__ __forceinline__ void bulk_load(uint32_t smem_dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(smem_dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+// the same; the lines read are the first to leave the L2 cache
+__device__ __forceinline__ void bulk_load_once(uint32_t smem_dst, const void* src, uint32_t bytes, uint32_t bar) {
+    uint64_t policy;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;"
+                 ::"r"(smem_dst), "l"(src), "r"(bytes), "r"(bar), "l"(policy) : "memory");
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
