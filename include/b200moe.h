@@ -287,8 +287,9 @@ int moe_rms_norm_backward(const moe_norm_grad_args* args, void* stream);
  * weights = p * scale, or with renormalize p / (sum of the chosen p + 1e-20) * scale.
  * logits [T, E] of `dtype` (bf16, f16, f32), row stride in elements; bias [E] bf16 or f32; ids int32 and weights f32
  * [T, top_k], in descending order of p + bias.  The order is the exact one of p + bias, ties to the lowest index.
- * A logit of -infinity or NaN (and a bias that is not finite) switches its expert off; where fewer than top_k are left
- * the id is -1 and the weight 0, and moe_permute_plan drops the pair.  E <= 1024, top_k <= min(32, E), n_group <= 32.
+ * A logit or bias of -infinity or NaN switches its expert off, +infinity counts as the largest finite number; where fewer
+ * than top_k experts are left the id is -1 and the weight 0, and moe_permute_plan drops the pair.  E <= 1024,
+ * top_k <= min(32, E), n_group <= 32, and the kept groups hold at least top_k experts.
  * The general form of moe_route_topk and moe_route_deepseek (fp32 logits; their fixed rules). */
 #define MOE_SCORE_SOFTMAX 0
 #define MOE_SCORE_SIGMOID 1

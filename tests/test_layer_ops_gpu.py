@@ -814,3 +814,47 @@ def test_refusals(ops, gg):
         with pytest.raises(error):
             call()
             pytest.fail(f"call {i} is not refused")
+
+
+# ------------------------------------------------------------------ offsets past 32 bits
+def test_offsets_past_32_bits(ops, gg):
+    """More than 2^32 bytes (and 2^31 elements) in front of the last rows, which are compared with the same rows alone."""
+    T, H, tail = 540000, 4096, 130
+    g = gen(90)
+    last = torch.zeros((tail, H)).normal_(generator=g).bfloat16().cuda()
+    w = torch.ones(H, device="cuda", dtype=torch.bfloat16)
+    x = torch.zeros((T, H), dtype=torch.bfloat16, device="cuda")
+    x[-tail:] = last
+    big, small = ops.rms_norm_quant(x, w), ops.rms_norm_quant(last, w)
+    assert torch.equal(big["q"][-tail:].view(torch.uint8), small["q"].view(torch.uint8)) and torch.equal(big["scales"][-tail:], small["scales"])
+    del big
+    dx, dw = ops.rms_norm_backward(x, x, w, torch.ones(T, device="cuda"))
+    dx0, _ = ops.rms_norm_backward(last, last, w, torch.ones(tail, device="cuda"))
+    assert torch.equal(dx[-tail:], dx0) and torch.isfinite(dw).all()
+    del dx
+    q, sf = ops.quant_fp4(x)
+    first = (T - tail) // 128 * 128                                       # whole tiles
+    q0, sf0 = ops.quant_fp4(x[first:])
+    assert torch.equal(q[first:], q0) and torch.equal(sf[first // 128:], sf0)
+    assert torch.equal(ops.unpack_fp4(q)[-tail:].view(torch.uint8), ops.unpack_fp4(q[-tail:].contiguous()).view(torch.uint8))
+    del q, sf
+    ids, wt = ops.route(x[:, :1024], 3)
+    ids0, wt0 = ops.route(last[:, :1024], 3)
+    assert torch.equal(ids[-tail:], ids0) and torch.equal(wt[-tail:], wt0)
+    z = x.view(-1, 1024)                                                  # dense rows for the gradient
+    gr = torch.ones((z.shape[0], 2), device="cuda")
+    at = torch.tensor([3, 700], dtype=torch.int32, device="cuda").expand(z.shape[0], 2).contiguous()
+    assert torch.equal(ops.route_backward(gr, z, at)[-tail:], ops.route_backward(gr[-tail:], z[-tail:], at[-tail:]))
+    del x, z, gr, at
+    # a product whose output passes 2^32 bytes
+    a, sfa, av = make_operand((), 256, 128, "mxfp4", 91)
+    b, sfb, bv = make_operand((2,), H, 128, "mxfp4", 92)
+    M = T // 128 * 128
+    rows = torch.zeros((M, 64), dtype=torch.uint8, device="cuda")
+    tiles = torch.zeros(ops.fp4_scale_shape(M, 128, "mxfp4"), dtype=torch.uint8, device="cuda")
+    rows[-256:], tiles[-2:] = a, sfa
+    layout = torch.zeros(M, dtype=torch.int32, device="cuda")
+    layout[-200:] = 1
+    d = torch.empty((M, H), dtype=torch.bfloat16, device="cuda")
+    gg.bind_contiguous_fp4(rows, tiles, b, sfb, d, layout, fmt="mxfp4")()
+    check_product(d[-256:], torch.zeros((256, H), dtype=torch.bfloat16), av, bv, layout[-256:].cpu(), None, torch.bfloat16)

@@ -261,8 +261,9 @@ def route(logits: torch.Tensor, top_k: int, score: str = "softmax", bias: torch.
     p = softmax or sigmoid of the logits; the experts are chosen by p + bias (bf16/f32 [E]) in its exact order, ties to the
     lowest index, and weighted by p (over its sum of the chosen with ``renormalize``) * scale.  With n_group > 1 only the
     topk_group best groups of E / n_group consecutive experts count; a group's score is its best p + bias ("max") or the
-    sum of its two best ("top2").  A logit of -inf or NaN switches its expert off; where fewer than top_k are left the id
-    is -1 and the weight 0, which :func:`permute_plan` drops."""
+    sum of its two best ("top2").  A logit or bias of -inf or NaN switches its expert off (+inf counts as the largest
+    number); where fewer than top_k experts are left the id is -1 and the weight 0, which :func:`permute_plan` drops.
+    E <= 1024, top_k <= 32, n_group <= 32."""
     _check_float(logits, "logits")
     T, E, ld = _rows(logits, "logits", 1)
     if bias is not None:
