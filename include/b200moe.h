@@ -346,7 +346,10 @@ typedef struct moe_fp4_quant_args {
     void* q;
     void* scales;
     int32_t groups, rows, src_rows, K, top_k, dtype, format, silu_mul, gate_first;
+    void* workspace;              /* 16-byte aligned, or NULL: not needed, but a call for which moe_quant_fp4_workspace_bytes is */
+    uint64_t workspace_bytes;     /* not 0 (src_pair with many rows for each of x) quantises x once with it, and copies rows */
 } moe_fp4_quant_args;
+size_t moe_quant_fp4_workspace_bytes(int32_t rows, int32_t src_rows, int32_t K, int32_t format);
 int moe_quant_fp4(const moe_fp4_quant_args* args, void* stream);
 
 /* The codes' values as e4m3 (which holds each of them): n_bytes of packed codes -> 2 * n_bytes of e4m3.  n_bytes % 8 == 0;

@@ -79,6 +79,18 @@ def test_quant_fp4_refuses(lib, kw, word):
     _refused(lib, "moe_quant_fp4", lib.Fp4QuantArgs(**(base | kw)), word)
 
 
+def test_quant_fp4_workspace(lib):
+    need = lib.lib().moe_quant_fp4_workspace_bytes
+    assert need(8192, 4096, 2048, 0) == 4096 * (1024 + 8 * 16) and need(8192, 4096, 2048, 1) == 4096 * (1024 + 8 * 8)
+    assert need(8192, 4097, 2048, 0) == 0 and need(4095, 1000, 2048, 0) == 0         # too few rows for one of x, too few values
+    for bad in ((-1, 1, 256, 0), (8192, 0, 2048, 0), (8192, 4096, 2000, 0), (8192, 4096, 2048, 2)):
+        assert need(*bad) == 0
+    base = dict(x=A16, x_stride=2048, src_pair=A16, q=A16, scales=A16, groups=1, rows=8192, src_rows=4096, K=2048, top_k=2, gate_first=1)
+    full = need(8192, 4096, 2048, 0)
+    for kw in (dict(workspace=A16, workspace_bytes=full - 1), dict(workspace=ODD, workspace_bytes=full)):
+        _refused(lib, "moe_quant_fp4", lib.Fp4QuantArgs(**(base | kw)), "workspace")
+
+
 @pytest.mark.parametrize("fn", ["moe_gg_fp4_contiguous", "moe_gg_fp4_masked"])
 @pytest.mark.parametrize("kw,word", [
     (dict(G=0), "G"), (dict(M=-1), "M"), (dict(N=20), "N=20"), (dict(K=64), "K=64"), (dict(format=5), "format"), (dict(d_dtype=2), "d_dtype"), (dict(ldd=48), "ldd"),

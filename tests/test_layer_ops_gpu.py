@@ -461,6 +461,55 @@ def test_quant_fp4_gather_leaves_padding_alone(ops, fmt):
     assert (b[~live] == 0x5A).all() and (q.cpu().numpy()[~live] == 0xA5).all()
 
 
+@pytest.mark.parametrize("fmt,dtype", [("nvfp4", "bf16"), ("mxfp4", "fp32"), ("nvfp4", "fp16")])
+def test_quant_fp4_gather_many_rows_of_each(ops, fmt, dtype):
+    """So many rows that x is quantised once and its rows are copied: ragged lengths, pairs that two rows have, skipped rows,
+    a stream of its own and a replayed graph that gets other pairs."""
+    from tirx_harness_b200 import _lib
+    T, K, top_k, rows = 900, 1152, 9, 7300
+    need = _lib.lib().moe_quant_fp4_workspace_bytes(rows, T, K, 0 if fmt == "nvfp4" else 1)
+    assert need > 0
+    x = torch.zeros((T, K + 16)).normal_(generator=gen(25)).to(DT[dtype])[:, :K]
+    x[3, 40] = math.nan
+    src = torch.randperm(T * top_k, generator=gen(26))[:rows].int()
+    src[100:140], src[200], src[rows - 1], src[300:500] = -1, 27, 27, 5
+    f = torch.tensor([7e-4], device="cuda") if fmt == "nvfp4" else None
+    xd, srcd = _cuda_strided(x), src.cuda()
+    shape = ops.fp4_scale_shape(rows, K, fmt)
+    q, sf = torch.full((rows, K // 2), 0xA5, dtype=torch.uint8, device="cuda"), torch.full(shape, 0x5A, dtype=torch.uint8, device="cuda")
+    rc, rb = quant32(x.float().numpy(), fmt, np.float32(7e-4) if fmt == "nvfp4" else 1.0)
+    block = 40 // BLOCK[fmt]                                       # the NaN's, which quant32 does not know
+    rb[3, block] = 0x7F if fmt == "nvfp4" else 0xFF
+    rc[3, block * BLOCK[fmt]:(block + 1) * BLOCK[fmt]] = 0
+
+    def check(src):
+        live, t = (src >= 0).numpy(), (src // top_k).clamp(min=0).long().numpy()
+        b = scale_bytes(sf, rows, K, fmt)
+        np.testing.assert_array_equal(b[live], rb[t][live])
+        assert same_codes(codes_of(q)[live], rc[t][live])
+        assert (b[~live] == 0x5A).all() and (q.cpu().numpy()[~live] == 0xA5).all()
+        full = scale_bytes(sf, shape[0] * 128, (K + 255) // 256 * 256, fmt)
+        assert not full[rows:].any() and not full[:rows][live][:, K // BLOCK[fmt]:].any()
+
+    def call():
+        ops.quant_fp4(xd, fmt=fmt, global_scale=f, src_pair=srcd, top_k=top_k, out=(q, sf))
+
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        call()
+    side.synchronize()
+    check(src)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        call()
+    other = src.clone()
+    other[src >= 0] = other[src >= 0].flip(0)
+    srcd.copy_(other)
+    graph.replay()
+    check(other)
+
+
 @pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
 @pytest.mark.parametrize("gate_first", [True, False])
 def test_quant_fp4_silu_mul(ops, fmt, gate_first):

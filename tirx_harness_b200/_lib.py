@@ -124,6 +124,7 @@ class Fp4QuantArgs(_c.Structure):
         ("src_pair", _c.c_void_p), ("q", _c.c_void_p), ("scales", _c.c_void_p),
         ("groups", _c.c_int32), ("rows", _c.c_int32), ("src_rows", _c.c_int32), ("K", _c.c_int32), ("top_k", _c.c_int32),
         ("dtype", _c.c_int32), ("format", _c.c_int32), ("silu_mul", _c.c_int32), ("gate_first", _c.c_int32),
+        ("workspace", _c.c_void_p), ("workspace_bytes", _c.c_uint64),
     ]
 
 
@@ -184,7 +185,7 @@ EXPORTS = (
     "moe_route_topk", "moe_route_deepseek", "moe_permute_workspace_bytes", "moe_permute_plan", "moe_permute_plan_static", "moe_permute",
     "moe_combine",
     "moe_rms_norm_quant", "moe_rms_norm_backward_workspace_bytes", "moe_rms_norm_backward", "moe_route", "moe_route_backward",
-    "moe_quant_fp4", "moe_unpack_fp4", "moe_gg_fp4_contiguous", "moe_gg_fp4_masked",
+    "moe_quant_fp4", "moe_quant_fp4_workspace_bytes", "moe_unpack_fp4", "moe_gg_fp4_contiguous", "moe_gg_fp4_masked",
     "moe_workspace_bytes", "moe_layer_forward", "moe_layer_workspace_view", "moe_device_status",
     "moe_alpha_workspace_bytes", "moe_alpha_forward", "moe_alpha_workspace_view",
     "moe_kg_workspace_bytes", "moe_kg_fp8_contiguous",
@@ -194,7 +195,8 @@ EXPORTS = (
     "moe_last_error", "moe_version",
 )
 _SIZE_T_RETURN = ("moe_gg_workspace_bytes", "moe_permute_workspace_bytes", "moe_workspace_bytes", "moe_ep_workspace_bytes",
-                  "moe_alpha_workspace_bytes", "moe_kg_workspace_bytes", "moe_rms_norm_backward_workspace_bytes")
+                  "moe_alpha_workspace_bytes", "moe_kg_workspace_bytes", "moe_rms_norm_backward_workspace_bytes",
+                  "moe_quant_fp4_workspace_bytes")
 
 
 # dtypes and modes of include/b200moe.h

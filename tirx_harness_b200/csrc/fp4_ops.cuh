@@ -89,13 +89,13 @@ __device__ __forceinline__ float silu_quick(float x) {
 
 constexpr int FP4_QUANT_THREADS = 256, FP4_QUANT_ROWS = 64;
 
-// NV: nvfp4, else mxfp4.  SILU: x holds gate and up, K columns each.
+// NV: nvfp4, else mxfp4.  SILU: x holds gate and up, K columns each.  BY_ROW: scales row after row, for copy_fp4_rows_kernel.
 // Block: 64 rows x 256 columns.  A thread takes 16 columns of a row at a time (a block of nvfp4, half a block of mxfp4) and
 // four such rows in all: of 16-bit inputs all four are loaded before the first is used, of the others two at a time.
 // Blocks per SM as measured (16384 x 7168 nvfp4: 3, 4, 5 blocks 66, 61, 66 us; mxfp4: 4, 5, 6 blocks 48, 46, 61 us; SiLU*mul of
 // 16384 x 2048: 2, 3, 4 blocks 42, 35, 39 us).  mxfp4 runs at memory's speed (45 us, 6.5 TB/s); nvfp4 has a division more per
 // value and is bound by its instructions (58 us, 5.2 TB/s).
-template <typename T, bool NV, bool SILU>
+template <typename T, bool NV, bool SILU, bool BY_ROW>
 __global__ void __launch_bounds__(FP4_QUANT_THREADS, sizeof(T) == 2 ? (SILU ? 3 : (NV ? 4 : 5)) : 2) quant_fp4_kernel(const Fp4QuantParams p) {
     constexpr int WORDS = NV ? 4 : 2;           // scale tiles of 256 columns
     constexpr int STEP = FP4_QUANT_THREADS / 16, ROWS = FP4_QUANT_ROWS / STEP, BATCH = sizeof(T) == 2 && !SILU ? ROWS : ROWS / 2;
@@ -187,12 +187,77 @@ __global__ void __launch_bounds__(FP4_QUANT_THREADS, sizeof(T) == 2 ? (SILU ? 3 
         }
     }
     __syncthreads();
+    if (BY_ROW) {
+        const int i = threadIdx.x;
+        if (i < FP4_QUANT_ROWS && r0 + i < p.rows) {
+            uint32_t* to = reinterpret_cast<uint32_t*>(p.sf) + ((long long)(r0 + i) * p.k_blocks + kb) * WORDS;
+            if (NV) *reinterpret_cast<uint4*>(to) = make_uint4(tile[0][i], tile[1][i], tile[WORDS - 2][i], tile[WORDS - 1][i]);
+            else *reinterpret_cast<uint2*>(to) = make_uint2(tile[0][i], tile[1][i]);
+        }
+        return;
+    }
     uint32_t* out = reinterpret_cast<uint32_t*>(p.sf) + (((long long)group * (row_pieces / (128 / FP4_QUANT_ROWS)) + (r0 >> 7)) * p.k_blocks + kb) * (WORDS * 128);
     for (int w = threadIdx.x; w < WORDS * FP4_QUANT_ROWS; w += FP4_QUANT_THREADS) {
         // neighbouring threads: the words of rows i and i + 32 lie side by side
         const int t = w / FP4_QUANT_ROWS, i = ((w & 1) << 5) + ((w % FP4_QUANT_ROWS) >> 1), r = r0 + i;
         // rows that are left alone keep their scales; those behind the last one are zero
         if (p.src == nullptr || r >= p.rows || __ldg(p.src + r) >= 0) out[t * 128 + (r & 31) * 4 + ((r >> 5) & 3)] = tile[t][i];
+    }
+}
+
+// Row r of (q, sf) <- row src[r] / top_k of (q0, sf0), x quantised once; the rows left alone are quant_fp4_kernel's.
+// Where every row of x goes to several rows, its quantisation (57 us for 16384 x 7168 nvfp4, bound by instructions) and this
+// copy (bound by the L2 cache: it reads and writes 147 MB each in 40 us for 32768 rows) beat a quantisation of each row:
+// 16384 x 7168 in 2 rows each 132 -> 97 us, 4096 x 7168 in 8 rows each 131 -> 48 us.  FP4_COPY_FROM says from where on.
+// Block: 64 rows x 1024 columns; a warp copies the 512 bytes of a row's codes and has eight rows under way.
+struct Fp4CopyParams {
+    const uint8_t* q0; const uint32_t* sf0;     // sf0: row after row
+    const int* src; int top_k;
+    uint8_t* q; uint32_t* sf;
+    int rows, src_rows, K, k_blocks, pieces;
+};
+constexpr int FP4_COPY_COLS = 1024;
+// Values from which a second kernel costs less than it saves (twice the rows of x or more; 3.7 million: 5.1 us without
+// and 6.4 us with it, 8.4 million: 7.4 and 6.6 us, 14.7 million: 11.3 and 7.4 us).  As many rows as x has: 70 us without, 82 with it.
+constexpr long long FP4_COPY_FROM = 1ll << 23;
+template <bool NV>
+__global__ void __launch_bounds__(FP4_QUANT_THREADS) copy_fp4_rows_kernel(const Fp4CopyParams p) {
+    constexpr int WARPS = FP4_QUANT_THREADS / 32, EACH = FP4_QUANT_ROWS / WARPS, WORDS = NV ? 4 : 2;
+    __shared__ int from[FP4_QUANT_ROWS];        // -1: leave the row alone; -2: zero scales
+    const int rb = blockIdx.x / p.pieces, piece = blockIdx.x - rb * p.pieces, r0 = rb * FP4_QUANT_ROWS;
+    if (threadIdx.x < FP4_QUANT_ROWS) {
+        const int r = r0 + threadIdx.x, pair = r < p.rows ? __ldg(p.src + r) : 0;
+        const int f = r < p.rows ? (pair >= 0 ? pair / p.top_k : -1) : -2;
+        from[threadIdx.x] = f < p.src_rows ? f : -2;
+    }
+    __syncthreads();
+    pdl_wait();
+    const int col = piece * (FP4_COPY_COLS / 2) + (threadIdx.x & 31) * 16, half = p.K >> 1;
+    uint4 c[EACH];
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+        const int f = from[(threadIdx.x >> 5) + j * WARPS];
+        if (f >= 0 && col < half) c[j] = *reinterpret_cast<const uint4*>(p.q0 + (long long)f * half + col);
+    }
+    // a thread takes a row's scales of 256 columns; neighbouring threads: rows i and i + 32, whose words lie side by side
+    static_assert(FP4_COPY_COLS / 256 * FP4_QUANT_ROWS == FP4_QUANT_THREADS);
+    const int kb = piece * (FP4_COPY_COLS / 256) + threadIdx.x / FP4_QUANT_ROWS;
+    const int i = ((threadIdx.x & 1) << 5) + ((threadIdx.x % FP4_QUANT_ROWS) >> 1), f = from[i], r = r0 + i;
+    if (f != -1 && kb < p.k_blocks) {
+        uint32_t w[WORDS] = {};
+        if (f >= 0) {
+            const uint32_t* at = p.sf0 + ((long long)f * p.k_blocks + kb) * WORDS;
+            if (NV) *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(at);
+            else *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(at);
+        }
+        uint32_t* out = p.sf + ((long long)(r >> 7) * p.k_blocks + kb) * (WORDS * 128) + (r & 31) * 4 + ((r >> 5) & 3);
+#pragma unroll
+        for (int t = 0; t < WORDS; ++t) out[t * 128] = w[t];
+    }
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+        const int row = (threadIdx.x >> 5) + j * WARPS;
+        if (from[row] >= 0 && col < half) __stcs(reinterpret_cast<uint4*>(p.q + (long long)(r0 + row) * half + col), c[j]);
     }
 }
 

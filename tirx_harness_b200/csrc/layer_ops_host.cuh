@@ -148,11 +148,13 @@ void launch_route_grad(const RouteGradParams& p, cudaStream_t st) {
 }
 
 template <typename T>
-void launch_quant_fp4(const Fp4QuantParams& p, bool nv, bool silu, dim3 grid, cudaStream_t st) {
-    if (nv && silu) quant_fp4_kernel<T, true, true><<<grid, FP4_QUANT_THREADS, 0, st>>>(p);
-    else if (nv) quant_fp4_kernel<T, true, false><<<grid, FP4_QUANT_THREADS, 0, st>>>(p);
-    else if (silu) quant_fp4_kernel<T, false, true><<<grid, FP4_QUANT_THREADS, 0, st>>>(p);
-    else quant_fp4_kernel<T, false, false><<<grid, FP4_QUANT_THREADS, 0, st>>>(p);
+void launch_quant_fp4(const Fp4QuantParams& p, bool nv, bool silu, bool by_row, dim3 grid, cudaStream_t st) {
+    if (by_row && nv) quant_fp4_kernel<T, true, false, true><<<grid, FP4_QUANT_THREADS, 0, st>>>(p);
+    else if (by_row) quant_fp4_kernel<T, false, false, true><<<grid, FP4_QUANT_THREADS, 0, st>>>(p);
+    else if (nv && silu) quant_fp4_kernel<T, true, true, false><<<grid, FP4_QUANT_THREADS, 0, st>>>(p);
+    else if (nv) quant_fp4_kernel<T, true, false, false><<<grid, FP4_QUANT_THREADS, 0, st>>>(p);
+    else if (silu) quant_fp4_kernel<T, false, true, false><<<grid, FP4_QUANT_THREADS, 0, st>>>(p);
+    else quant_fp4_kernel<T, false, false, false><<<grid, FP4_QUANT_THREADS, 0, st>>>(p);
 }
 
 // 1-D array of scale tiles as 64-bit words, box = one chunk (the scales of 128 rows x 256 values)
@@ -381,6 +383,11 @@ int moe_route_backward(const moe_route_grad_args* a, void* stream) {
     return MOE_OK;
 }
 
+size_t moe_quant_fp4_workspace_bytes(int32_t rows, int32_t src_rows, int32_t K, int32_t format) {
+    if (src_rows <= 0 || K <= 0 || K % 128 || rows < 2ll * src_rows || (long long)rows * K < FP4_COPY_FROM || (format != MOE_FP4_NV && format != MOE_FP4_MX)) return 0;
+    return align256((size_t)src_rows * (size_t)(K / 2)) + align256((size_t)src_rows * ((K + 255ll) / 256) * (format == MOE_FP4_NV ? 16 : 8));
+}
+
 int moe_quant_fp4(const moe_fp4_quant_args* a, void* stream) {
     if (!a) return fail(MOE_ERR_INVALID, "args is NULL");
     if (a->groups <= 0 || a->groups > 65535 || a->rows < 0 || a->src_rows < 0 || a->K <= 0 || a->K % 128)
@@ -395,17 +402,28 @@ int moe_quant_fp4(const moe_fp4_quant_args* a, void* stream) {
     const int64_t cols = a->silu_mul ? 2ll * a->K : a->K;
     if (!aligned16(a->x) || a->x_stride < cols || a->x_stride % 8) return fail(MOE_ERR_INVALID, "x must be 16-byte aligned with a row stride that covers its columns and is a multiple of 8");
     if (!aligned16(a->q) || !aligned16(a->scales)) return fail(MOE_ERR_INVALID, "q and scales must be 16-byte aligned");
-    Fp4QuantParams p;
+    Fp4QuantParams p = {};
     p.x = a->x; p.x_stride = a->x_stride; p.factor = a->factor; p.factor_stride = a->factor_stride; p.src = a->src_pair; p.top_k = a->top_k;
     p.q = static_cast<uint8_t*>(a->q); p.sf = static_cast<uint8_t*>(a->scales); p.rows = a->rows; p.K = a->K;
     p.gate_first = a->gate_first ? 1 : 0; p.src_rows = a->src_rows; p.k_blocks = (a->K + 255) / 256;
-    const long long blocks = (long long)((a->rows + 127) / 128) * (128 / FP4_QUANT_ROWS) * p.k_blocks;
-    if (blocks > 0x7FFFFFFFll) return fail(MOE_ERR_INVALID, "rows x K exceeds what one call covers");
-    const dim3 grid((unsigned)blocks, a->groups, 1);
-    with_dtype(a->dtype, [&](auto t) {
-        launch_quant_fp4<decltype(t)>(p, a->format == MOE_FP4_NV, a->silu_mul != 0, grid, static_cast<cudaStream_t>(stream));
-    });
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const size_t need = a->src_pair && !a->silu_mul ? moe_quant_fp4_workspace_bytes(a->rows, a->src_rows, a->K, a->format) : 0;
+    const bool copy = need > 0 && a->workspace != nullptr;
+    if (copy) {
+        if (!aligned16(a->workspace) || a->workspace_bytes < need) return fail(MOE_ERR_INVALID, "workspace too small or not 16-byte aligned (moe_quant_fp4_workspace_bytes)");
+        p.src = nullptr; p.rows = a->src_rows; p.q = static_cast<uint8_t*>(a->workspace); p.sf = p.q + align256((size_t)a->src_rows * (size_t)(a->K / 2));
+    }
+    const auto row_pieces = [](int rows) { return (long long)((rows + 127ll) / 128) * (128 / FP4_QUANT_ROWS); };
+    if (row_pieces(a->rows) * p.k_blocks > 0x7FFFFFFFll) return fail(MOE_ERR_INVALID, "rows x K exceeds what one call covers");
+    const dim3 grid((unsigned)(row_pieces(p.rows) * p.k_blocks), a->groups, 1);
+    with_dtype(a->dtype, [&](auto t) { launch_quant_fp4<decltype(t)>(p, a->format == MOE_FP4_NV, a->silu_mul != 0, copy, grid, st); });
     CUDA_TRY(cudaGetLastError());
+    if (copy) {
+        const Fp4CopyParams c = {p.q, reinterpret_cast<const uint32_t*>(p.sf), a->src_pair, a->top_k, static_cast<uint8_t*>(a->q), static_cast<uint32_t*>(a->scales),
+                                 a->rows, a->src_rows, a->K, p.k_blocks, (a->K + FP4_COPY_COLS - 1) / FP4_COPY_COLS};
+        CUDA_TRY(launch_pdl(a->format == MOE_FP4_NV ? copy_fp4_rows_kernel<true> : copy_fp4_rows_kernel<false>, dim3((unsigned)(row_pieces(a->rows) * c.pieces)),
+                            dim3(FP4_QUANT_THREADS), 0, st, c));
+    }
     return MOE_OK;
 }
 

@@ -356,8 +356,12 @@ def quant_fp4(x: torch.Tensor, fmt: str = "nvfp4", global_scale: torch.Tensor | 
         q, s = make(q_shape, dtype=torch.uint8), make(s_shape, dtype=torch.uint8)
     if G == 0 or rows == 0:
         return q, s
+    ws, n = None, 0
+    if rows > src_rows and act is None:                      # gathered with several rows for one of x: it is quantised once
+        n = _lib.lib().moe_quant_fp4_workspace_bytes(_i32(rows), _i32(src_rows), _i32(K), _i32(_FP4_FORMAT[fmt]))
+        ws = x.new_empty(n, dtype=torch.uint8) if n else None
     _launch(_lib.FP4_QUANT, x.device, x.data_ptr(), ld, _p(global_scale), gs, _p(src_pair), q.data_ptr(), s.data_ptr(), G, rows, src_rows, K,
-            top_k, _DTYPE[x.dtype], _FP4_FORMAT[fmt], 1 if act is not None else 0, 1 if gate_first else 0)
+            top_k, _DTYPE[x.dtype], _FP4_FORMAT[fmt], 1 if act is not None else 0, 1 if gate_first else 0, _p(ws), n)
     return q, s
 
 
