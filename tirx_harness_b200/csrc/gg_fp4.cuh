@@ -59,16 +59,14 @@ namespace f4 {
 constexpr int BM = 128, BKB = 128;                        // rows per CTA; bytes of K per stage (256 values)
 constexpr int THREADS = 384;
 constexpr int TMEM_COLS = 512;
-template <bool NV, int TN> struct Cfg {
+constexpr int TN = 256;                                   // columns of a tile
+template <bool NV> struct Cfg {
     static constexpr int SF_CHUNK = NV ? 2048 : 1024;     // scales of 128 rows x 256 values
     static constexpr int A_BYTES = BM * BKB, B_BYTES = (TN / 2) * BKB;
     static constexpr int SF_BYTES = 3 * SF_CHUNK;         // this CTA's rows, the tile's columns (2 x 128)
-    static constexpr int STAGES = (TN == 256 && NV) ? 5 : 6;
-    static constexpr int ACCS = TN <= 192 ? 2 : 1;
-    static constexpr int SFA_COLS = NV ? 16 : 8, SF_COLS = 3 * SFA_COLS;
-    static constexpr int SF_BASE = ACCS * TN;
-    static constexpr int SF_FIT = (TMEM_COLS - SF_BASE) / SF_COLS;
-    static constexpr int SF_BUFS = SF_FIT < STAGES ? SF_FIT : STAGES;
+    static constexpr int STAGES = NV ? 5 : 6;
+    static constexpr int SFA_COLS = NV ? 16 : 8, SF_COLS = 3 * SFA_COLS;      // TMEM: the accumulator, then a stage's scales
+    static_assert(TN + STAGES * SF_COLS <= TMEM_COLS);
     static constexpr int OFF_B = STAGES * A_BYTES;
     static constexpr int OFF_SF = OFF_B + STAGES * B_BYTES;
     static constexpr int OFF_BARS = OFF_SF + STAGES * SF_BYTES;
@@ -215,26 +213,26 @@ template <bool MASKED> struct Fp4Sched {
     }
 };
 
-template <bool NV, bool MASKED, int TN>
+template <bool NV, bool MASKED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(f4::THREADS, 1)
 gg_fp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                    const __grid_constant__ CUtensorMap tmap_sfa, const __grid_constant__ CUtensorMap tmap_sfb,
                    const GGFp4Params p, const GGParams sp, int* status) {
     using namespace f4;
-    using C = Cfg<NV, TN>;
-    constexpr int STAGES = C::STAGES, ACCS = C::ACCS;
+    using C = Cfg<NV>;
+    constexpr int STAGES = C::STAGES;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BARS);
-    // [0,S) full (leader's used), [S,2S) empty, then 2 tmem_full, 2 tmem_empty (leader's used)
-    uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 4);
+    // [0,S) full (leader's used), [S,2S) empty, then tmem_full, tmem_empty (leader's used)
+    uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_base_slot + 1);
     int* prefix = reinterpret_cast<int*>(smem + C::OFF_PREFIX);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);       // a value the compiler knows to be warp-uniform
     const int lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();
     const uint32_t full_bar = smem_u32(bars), empty_bar = smem_u32(bars + STAGES);
-    const uint32_t tfull_bar = smem_u32(bars + 2 * STAGES), tempty_bar = smem_u32(bars + 2 * STAGES + 2);
+    const uint32_t tfull_bar = smem_u32(bars + 2 * STAGES), tempty_bar = smem_u32(bars + 2 * STAGES + 1);
     const uint32_t leader_full_bar = map_to_cta(full_bar, 0), leader_tempty_bar = map_to_cta(tempty_bar, 0);
 
     if (threadIdx.x == 0) {
@@ -242,10 +240,8 @@ gg_fp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
             mbar_init(full_bar + 8 * s, 1);
             mbar_init(empty_bar + 8 * s, 1);
         }
-        for (int a = 0; a < 2; ++a) {
-            mbar_init(tfull_bar + 8 * a, 1);
-            mbar_init(tempty_bar + 8 * a, 16);        // the 16 epilogue warps of the pair
-        }
+        mbar_init(tfull_bar, 1);
+        mbar_init(tempty_bar, 16);                    // the 16 epilogue warps of the pair
         *abort_flag = 0;
         fence_mbar_init();
         tma_prefetch_desc(&tmap_a);
@@ -328,26 +324,23 @@ gg_fp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
             // ------------------------------------------------ MMA issuer (leader)
             Fp4Sched<MASKED> sched(p, sp, prefix, listed_tiles, lane, rank);
             Tile tile, next_tile;
-            uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0, sfb_buf = 0;
+            uint32_t stage = 0, phase = 0, acc_phase = 0;
             bool ok = true;
             const uint64_t adesc0 = make_smem_desc_sw128(smem_u32(smem));
             const uint64_t bdesc0 = make_smem_desc_sw128(smem_u32(smem + C::OFF_B));
             const uint64_t sdesc0 = make_sf_desc(smem_u32(smem + C::OFF_SF));
             bool have = sched.next(tile), have_next = false;
             while (ok && have) {
-                ok = mbar_wait_warp(tempty_bar + 8 * acc, acc_phase ^ 1, abort_flag, status, STATUS_TIMEOUT_TMEM_EMPTY);
+                ok = mbar_wait_warp(tempty_bar, acc_phase ^ 1, abort_flag, status, STATUS_TIMEOUT_TMEM_EMPTY);
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t idesc = make_idesc_fp4<NV>(2 * BM, tile_cols(tile.n_blk), 0);
-                const uint32_t tmem_d = tmem_base + acc * TN;
-                // a tile that starts inside a 128-column scale block: its scales are one column per 32 columns further on
-                const uint32_t shift = (uint32_t)((tile.n_blk * TN) & 127) >> 5;
                 for (int kb = 0; kb < KB; ++kb) {
                     ok = mbar_wait_warp(full_bar + 8 * stage, phase, abort_flag, status, STATUS_TIMEOUT_SMEM_FULL);
                     if (!ok) break;
                     tc_fence_after();
                     if (elect_one_sync()) {
-                        const uint32_t tsf = tmem_base + C::SF_BASE + sfb_buf * C::SF_COLS;
+                        const uint32_t tsf = tmem_base + TN + stage * C::SF_COLS;
                         const uint64_t sd = sdesc0 + stage * (C::SF_BYTES >> 4);
                         constexpr int TILES = C::SFA_COLS / 4;
 #pragma unroll
@@ -361,19 +354,18 @@ gg_fp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
                         for (int j = 0; j < 4; ++j) {
                             const int w = NV ? j : j >> 1;
                             const uint32_t id = NV ? 0u : (uint32_t)(j & 1) * 2u;
-                            umma_fp4_pair<NV>(tmem_d, adesc + 2 * j, bdesc + 2 * j, idesc | (id << 4) | (id << 29), tsf + 4 * w,
-                                              tsf + C::SFA_COLS + 8 * w + shift, kb > 0 || j > 0 ? 1u : 0u);
+                            umma_fp4_pair<NV>(tmem_base, adesc + 2 * j, bdesc + 2 * j, idesc | (id << 4) | (id << 29), tsf + 4 * w,
+                                              tsf + C::SFA_COLS + 8 * w, kb > 0 || j > 0 ? 1u : 0u);
                         }
                         umma_commit_pair(empty_bar + 8 * stage, 3);
-                        if (kb == KB - 1) umma_commit_pair(tfull_bar + 8 * acc, 3);
+                        if (kb == KB - 1) umma_commit_pair(tfull_bar, 3);
                     }
                     if (++stage == STAGES) { stage = 0; phase ^= 1; }
-                    if (++sfb_buf == C::SF_BUFS) sfb_buf = 0;
                     if (kb == 0) have_next = sched.next(next_tile);
                 }
                 tile = next_tile;
                 have = have_next;
-                if (++acc == ACCS) { acc = 0; acc_phase ^= 1; }
+                acc_phase ^= 1;
             }
         }
     } else {
@@ -385,17 +377,17 @@ gg_fp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
         const int m_end = !MASKED && p.rows_used ? min(p.M, __ldg(p.rows_used)) : p.M;       // rows behind it are not written
         Fp4Sched<MASKED> sched(p, sp, prefix, listed_tiles, lane, rank);
         Tile tile;
-        uint32_t acc = 0, acc_phase = 0;
+        uint32_t acc_phase = 0;
         bool ok = true;
         while (ok && sched.next(tile)) {
             const int n0 = tile.n_blk * TN + half * COLS;
             const int row = tile.m0 + row_in_tile;
             const bool row_valid = MASKED ? row_in_tile < tile.rows : (row < m_end && __ldg(p.layout + row) == tile.g);
             const float alpha = p.alpha ? __ldg(p.alpha + tile.g * p.alpha_stride) : 1.0f;
-            ok = mbar_wait_warp(tfull_bar + 8 * acc, acc_phase, abort_flag, status, STATUS_TIMEOUT_TMEM_FULL);
+            ok = mbar_wait_warp(tfull_bar, acc_phase, abort_flag, status, STATUS_TIMEOUT_TMEM_FULL);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t taddr = tmem_base + (uint32_t(quarter * 32) << 16) + acc * TN + half * COLS;
+            const uint32_t taddr = tmem_base + (uint32_t(quarter * 32) << 16) + half * COLS;
             uint32_t v[CHUNKS][32];
 #pragma unroll
             for (int c = 0; c < CHUNKS; ++c) tmem_ld_32x32b_x32(taddr + c * 32, v[c]);
@@ -403,8 +395,8 @@ gg_fp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
             for (int c = 0; c < CHUNKS; ++c) tmem_ld_wait(v[c]);
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(leader_tempty_bar + 8 * acc);
-            if (++acc == ACCS) { acc = 0; acc_phase ^= 1; }
+            if (lane == 0) mbar_arrive_cluster(leader_tempty_bar);
+            acc_phase ^= 1;
             if (!row_valid) continue;
             if (p.d_f32) {
                 float* drow = static_cast<float*>(p.d) + (long long)row * p.ldd + n0;

@@ -172,32 +172,32 @@ int encode_scale_chunks(CUtensorMap* map, const void* base, uint64_t bytes, uint
     return MOE_OK;
 }
 
-template <bool NV, bool MASKED, int TN>
+template <bool NV, bool MASKED>
 int launch_fp4_pair(const GGFp4Params& p, long long rows_total, DeviceInfo* di, cudaStream_t st) {
-    using C = f4::Cfg<NV, TN>;
+    using C = f4::Cfg<NV>;
     CUtensorMap ta, tb, tsa, tsb;
     int rc;
     const uint64_t kt = (uint64_t)p.kt * 512;
     if ((rc = encode_fp8_kmajor(&ta, p.a, (uint64_t)rows_total, (uint64_t)p.K / 2, f4::BM)) != MOE_OK) return rc;
-    if ((rc = encode_fp8_kmajor(&tb, p.b, (uint64_t)p.G * p.N, (uint64_t)p.K / 2, TN / 2)) != MOE_OK) return rc;
+    if ((rc = encode_fp8_kmajor(&tb, p.b, (uint64_t)p.G * p.N, (uint64_t)p.K / 2, f4::TN / 2)) != MOE_OK) return rc;
     if ((rc = encode_scale_chunks(&tsa, p.sfa, (uint64_t)(MASKED ? p.G : 1) * p.a_tiles * kt, C::SF_CHUNK)) != MOE_OK) return rc;
     if ((rc = encode_scale_chunks(&tsb, p.sfb, (uint64_t)p.G * p.b_tiles * kt, C::SF_CHUNK)) != MOE_OK) return rc;
     GGParams sp = {};
     sp.layout = p.layout; sp.rows_used = p.rows_used; sp.G = p.G; sp.M = p.M; sp.N = p.N;
-    sp.num_n_blocks = (p.N + TN - 1) / TN;
+    sp.num_n_blocks = (p.N + f4::TN - 1) / f4::TN;
     // row blocks that sorted rows can fill (more tiles than this only make the pairs take more than one each)
     const long long blocks = MASKED ? (long long)p.G * ((p.M + 255) / 256) : (p.M + 255) / 256 + (p.G < p.M ? p.G : p.M) - 1;
     const long long tiles = blocks * sp.num_n_blocks;
     const int pairs = (int)(tiles < di->max_pairs ? tiles : di->max_pairs);
     static std::atomic<uint64_t> done{0};
-    if ((rc = raise_smem(gg_fp4_pair_kernel<NV, MASKED, TN>, C::SMEM_BYTES, done)) != MOE_OK) return rc;
-    gg_fp4_pair_kernel<NV, MASKED, TN><<<2 * pairs, f4::THREADS, C::SMEM_BYTES, st>>>(ta, tb, tsa, tsb, p, sp, di->status);
+    if ((rc = raise_smem(gg_fp4_pair_kernel<NV, MASKED>, C::SMEM_BYTES, done)) != MOE_OK) return rc;
+    gg_fp4_pair_kernel<NV, MASKED><<<2 * pairs, f4::THREADS, C::SMEM_BYTES, st>>>(ta, tb, tsa, tsb, p, sp, di->status);
     CUDA_TRY(cudaGetLastError());
     return MOE_OK;
 }
-template <bool NV, int TN>
+template <bool NV>
 int launch_fp4_pair_layout(const GGFp4Params& p, long long rows_total, DeviceInfo* di, cudaStream_t st) {
-    return p.masked ? launch_fp4_pair<NV, true, TN>(p, rows_total, di, st) : launch_fp4_pair<NV, false, TN>(p, rows_total, di, st);
+    return p.masked ? launch_fp4_pair<NV, true>(p, rows_total, di, st) : launch_fp4_pair<NV, false>(p, rows_total, di, st);
 }
 
 // the most (group, chunk of NT rows) that can have rows
@@ -274,7 +274,7 @@ int launch_gg_fp4(const moe_gg_fp4_args* a, bool masked, void* stream) {
     const bool one_round = row_chunks * ((a->N + 127) / 128) <= di->num_sms && fp4_few_entries(p, 128) <= ff::LIST_CAP &&
                            (masked || a->M <= ff::MAX_ROWS) && a->G <= (1 << 20);
     if ((a->M <= 128 && a->G <= (1 << 20)) || one_round) return nv ? launch_fp4_few<true, 128>(p, rows_total, di, st) : launch_fp4_few<false, 128>(p, rows_total, di, st);
-    return nv ? launch_fp4_pair_layout<true, 256>(p, rows_total, di, st) : launch_fp4_pair_layout<false, 256>(p, rows_total, di, st);
+    return nv ? launch_fp4_pair_layout<true>(p, rows_total, di, st) : launch_fp4_pair_layout<false>(p, rows_total, di, st);
 }
 
 }  // namespace
