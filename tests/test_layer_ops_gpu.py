@@ -442,6 +442,20 @@ def test_quant_fp4_not_finite_and_extreme(ops):
         assert same_codes(c[2:], ref)
 
 
+@pytest.mark.parametrize("factor", [1e-10, 1e-36, 1e36, 2.0**-126, 1.5])
+def test_quant_fp4_far_away_factors(ops, factor):
+    """Values that overflow against the largest scale keep their sign and become 6; scales that come out as zero leave zeros;
+    factors at the ends of the range are divided by like any other."""
+    g = gen(27)
+    x = torch.zeros((8, 256)).normal_(generator=g) * 10.0 ** torch.arange(-32, 48, 10).float().clamp(max=37)[:, None]
+    q, sf = ops.quant_fp4(x.cuda(), global_scale=torch.tensor([factor], device="cuda"))
+    rc, rb = quant32(x.numpy(), "nvfp4", np.float32(factor))
+    np.testing.assert_array_equal(scale_bytes(sf, 8, 256, "nvfp4"), rb)
+    live = np.repeat(rb, 16, 1) != 0
+    assert same_codes(codes_of(q)[live], rc[live])
+    assert not E2M1[codes_of(q)][~live].any()
+
+
 @pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
 def test_quant_fp4_gather_leaves_padding_alone(ops, fmt):
     T, K, top_k = 50, 256, 3

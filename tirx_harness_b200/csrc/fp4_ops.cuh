@@ -87,25 +87,58 @@ __device__ __forceinline__ float silu_quick(float x) {
     return x * r;
 }
 
+// One nvfp4 block by CUDA's division: its codes, and its scale byte as the result.  For factors at the ends of the range and
+// for values that overflow against the largest scale; a block that is not finite keeps the zeros it has.  Behind the loop over
+// the rows: 68 such divisions inside it took registers from every block (16384 x 7168: 58 us instead of 54).
+template <typename T, bool SILU>
+__device__ __forceinline__ uint8_t divided_block(const T* gate, const T* up, float g, uint8_t* q) {
+    f32x2 v[2][4];
+    float amax = 0.0f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        unpack8(load8(gate + 8 * h), v[h]);
+        if (SILU) {
+            f32x2 w[4];
+            unpack8(load8(up + 8 * h), w);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[h][j] = mul2(pack_f32x2(silu_quick(lo2(v[h][j])), silu_quick(hi2(v[h][j]))), w[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) amax = amax_nan(amax_nan(amax, lo2(v[h][j])), hi2(v[h][j]));
+    }
+    if (!(amax < INFINITY)) return 0x7F;
+    const __nv_fp8_storage_t byte = __nv_cvt_float_to_fp8(fminf(__fdiv_rn(amax, __fmul_rn(6.0f, g)), 448.0f), __NV_SATFINITE, __NV_E4M3);
+    const float unit = __fmul_rn(__half2float(__half(__nv_cvt_fp8_to_halfraw(byte, __NV_E4M3))), g);
+    if (unit > 0.0f) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j >> 2][j & 3] = pack_f32x2(__fdiv_rn(lo2(v[j >> 2][j & 3]), unit), __fdiv_rn(hi2(v[j >> 2][j & 3]), unit));
+        *reinterpret_cast<uint2*>(q) = make_uint2(pack8_e2m1(v[0]), pack8_e2m1(v[1]));
+    }
+    return byte;
+}
+
 constexpr int FP4_QUANT_THREADS = 256, FP4_QUANT_ROWS = 64;
 
 // NV: nvfp4, else mxfp4.  SILU: x holds gate and up, K columns each.  BY_ROW: scales row after row, for copy_fp4_rows_kernel.
 // Block: 64 rows x 256 columns.  A thread takes 16 columns of a row at a time (a block of nvfp4, half a block of mxfp4) and
 // four such rows in all: of 16-bit inputs all four are loaded before the first is used, of the others two at a time.
-// Blocks per SM as measured (16384 x 7168 nvfp4: 3, 4, 5 blocks 66, 61, 66 us; mxfp4: 4, 5, 6 blocks 48, 46, 61 us; SiLU*mul of
-// 16384 x 2048: 2, 3, 4 blocks 42, 35, 39 us).  mxfp4 runs at memory's speed (45 us, 6.5 TB/s); nvfp4 has a division more per
-// value and is bound by its instructions (58 us, 5.2 TB/s).
+// Blocks per SM as measured (16384 x 7168 nvfp4: 3, 4, 5 blocks 59, 55, 53 us; mxfp4: 4, 5, 6 blocks 48, 46, 61 us; SiLU*mul of
+// 16384 x 2048: 2, 3, 4 blocks 42, 31, 31 us).  mxfp4 runs at memory's speed (45 us, 6.5 TB/s); nvfp4 has a division more per
+// value and is bound by its instructions (53 us, 5.7 TB/s).  What it divides by has one value per scale byte: the block tables
+// them with their reciprocals.
 template <typename T, bool NV, bool SILU, bool BY_ROW>
-__global__ void __launch_bounds__(FP4_QUANT_THREADS, sizeof(T) == 2 ? (SILU ? 3 : (NV ? 4 : 5)) : 2) quant_fp4_kernel(const Fp4QuantParams p) {
+__global__ void __launch_bounds__(FP4_QUANT_THREADS, sizeof(T) == 2 ? (SILU ? 3 : 5) : 2) quant_fp4_kernel(const Fp4QuantParams p) {
     constexpr int WORDS = NV ? 4 : 2;           // scale tiles of 256 columns
     constexpr int STEP = FP4_QUANT_THREADS / 16, ROWS = FP4_QUANT_ROWS / STEP, BATCH = sizeof(T) == 2 && !SILU ? ROWS : ROWS / 2;
     __shared__ uint32_t tile[WORDS][FP4_QUANT_ROWS];
+    __shared__ float2 units[NV ? 128 : 1];      // of a scale byte: minus s g, and 1 / (s g), 0 for the scale zero
     const int group = blockIdx.y, row_pieces = ((p.rows + 127) >> 7) * (128 / FP4_QUANT_ROWS);
     const int rb = blockIdx.x / p.k_blocks, kb = blockIdx.x - rb * p.k_blocks;
     const int r0 = rb * FP4_QUANT_ROWS, i0 = threadIdx.x >> 4;
     const int seg = threadIdx.x & 15, col = kb * 256 + seg * 16;
     const float g = p.factor ? __ldg(p.factor + group * p.factor_stride) : 1.0f;
     const float g6 = __fmul_rn(6.0f, g), r6 = __frcp_rn(g6);
+    const bool near = g > 1e-27f && g < 1e26f;  // div_by can divide by 6 g and by every scale but zero
     const T* xg = static_cast<const T*>(p.x) + (long long)group * p.src_rows * p.x_stride + col;
     const int gate = SILU && !p.gate_first ? p.K : 0, up = p.gate_first ? p.K : 0;
     int src[ROWS];
@@ -119,6 +152,7 @@ __global__ void __launch_bounds__(FP4_QUANT_THREADS, sizeof(T) == 2 ? (SILU ? 3 
         if (p.src && src[k] >= 0) src[k] = src[k] / p.top_k;
         if (src[k] >= p.src_rows) src[k] = -1;
     }
+    unsigned again = 0;                         // rows whose block is left to divided_block
 #pragma unroll
     for (int b = 0; b < ROWS; b += BATCH) {
         Raw8<T> x[BATCH][2], u[SILU ? BATCH : 1][2];
@@ -132,6 +166,13 @@ __global__ void __launch_bounds__(FP4_QUANT_THREADS, sizeof(T) == 2 ? (SILU ? 3 
                 u[k][0] = load8(row + up);
                 u[k][1] = load8(row + up + 8);
             }
+        }
+        if (NV && b == 0) {                     // while the rows are on their way
+            if (threadIdx.x < 128) {
+                const float unit = __fmul_rn(__half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)threadIdx.x, __NV_E4M3))), g);
+                units[threadIdx.x] = make_float2(-unit, unit > 0.0f ? __frcp_rn(unit) : 0.0f);
+            }
+            __syncthreads();
         }
 #pragma unroll
         for (int k = 0; k < BATCH; ++k) {
@@ -157,34 +198,37 @@ __global__ void __launch_bounds__(FP4_QUANT_THREADS, sizeof(T) == 2 ? (SILU ? 3 
             if (!NV) amax = amax_nan(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
             uint32_t byte = 0;
             if (live) {
-                const bool finite = amax < INFINITY;
+                uint2 codes;
                 if (NV) {
-                    // a quotient that overflows in div_by becomes NaN, which fminf takes for 448 too
-                    const float t = div_ok(g6) ? lo2(div_by(both(amax), both(-g6), both(r6))) : __fdiv_rn(amax, g6);
-                    byte = finite ? __nv_cvt_float_to_fp8(fminf(t, 448.0f), __NV_SATFINITE, __NV_E4M3) : 0x7Fu;
-                    const float unit = __fmul_rn(__half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3))), g);
-                    if (finite && unit > 0.0f) {
-                        div8(v[0], unit);
-                        div8(v[1], unit);
-                    } else {
+                    const float q = __fmul_rn(amax, r6), t = __fmaf_rn(__fmaf_rn(-g6, q, amax), r6, q);       // amax / (6 g)
+                    const bool fit = near && t < 1e30f;     // false for a NaN too
+                    if (!fit) again |= 1u << (b + k);
+                    byte = fit ? __nv_cvt_float_to_fp8(fminf(t, 448.0f), __NV_SATFINITE, __NV_E4M3) : 0x7Fu;
+                    const float2 of = units[byte];
+                    const f32x2 minus = both(of.x), r = both(of.y);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) v[0][j] = v[1][j] = 0;
-                    }
+                    for (int j = 0; j < 8; ++j) v[j >> 2][j & 3] = div_by(v[j >> 2][j & 3], minus, r);
+                    codes = make_uint2(pack8_e2m1(v[0]), pack8_e2m1(v[1]));
+                    if (!fit) codes = make_uint2(0u, 0u);
                 } else {
+                    const bool finite = amax < INFINITY;
                     byte = finite ? (uint32_t)max((int)(__float_as_uint(amax) >> 23) - 2, 0) : 0xFFu;
                     const f32x2 inv = both(__uint_as_float((254u - byte) << 23));                 // 2^(127 - byte), exact
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        v[0][j] = finite ? mul2(v[0][j], inv) : 0;
-                        v[1][j] = finite ? mul2(v[1][j], inv) : 0;
-                    }
+                    for (int j = 0; j < 8; ++j) v[j >> 2][j & 3] = finite ? mul2(v[j >> 2][j & 3], inv) : 0;
+                    codes = make_uint2(pack8_e2m1(v[0]), pack8_e2m1(v[1]));
                 }
-                *reinterpret_cast<uint2*>(p.q + ((long long)group * p.rows + r0 + i) * (p.K >> 1) + (col >> 1)) =
-                    make_uint2(pack8_e2m1(v[0]), pack8_e2m1(v[1]));
+                *reinterpret_cast<uint2*>(p.q + ((long long)group * p.rows + r0 + i) * (p.K >> 1) + (col >> 1)) = codes;
             }
             const int blk = NV ? seg : seg >> 1;            // block of these 256 columns
             if (NV || !(seg & 1)) reinterpret_cast<uint8_t*>(&tile[blk >> 2][i])[blk & 3] = (uint8_t)byte;
         }
+    }
+    for (; again; again &= again - 1) {
+        const int i = i0 + (__ffs(again) - 1) * STEP, r = r0 + i;
+        const T* row = xg + (p.src ? __ldg(p.src + r) / p.top_k : r) * p.x_stride;
+        reinterpret_cast<uint8_t*>(&tile[seg >> 2][i])[seg & 3] =
+            divided_block<T, SILU>(row + gate, row + up, g, p.q + ((long long)group * p.rows + r) * (p.K >> 1) + (col >> 1));
     }
     __syncthreads();
     if (BY_ROW) {
@@ -206,9 +250,9 @@ __global__ void __launch_bounds__(FP4_QUANT_THREADS, sizeof(T) == 2 ? (SILU ? 3 
 }
 
 // Row r of (q, sf) <- row src[r] / top_k of (q0, sf0), x quantised once; the rows left alone are quant_fp4_kernel's.
-// Where every row of x goes to several rows, its quantisation (57 us for 16384 x 7168 nvfp4, bound by instructions) and this
-// copy (bound by the L2 cache: it reads and writes 147 MB each in 40 us for 32768 rows) beat a quantisation of each row:
-// 16384 x 7168 in 2 rows each 132 -> 97 us, 4096 x 7168 in 8 rows each 131 -> 48 us.  FP4_COPY_FROM says from where on.
+// Where every row of x goes to several rows, its quantisation (53 us for 16384 x 7168 nvfp4, bound by instructions) and this
+// copy (bound by the L2 cache: it reads and writes 132 MB each in 36 us for 32768 rows) beat a quantisation of each row:
+// 16384 x 7168 in 2 rows each 113 -> 89 us, 4096 x 7168 in 8 rows each 108 -> 46 us.  FP4_COPY_FROM says from where on.
 // Block: 64 rows x 1024 columns; a warp copies the 512 bytes of a row's codes and has eight rows under way.
 struct Fp4CopyParams {
     const uint8_t* q0; const uint32_t* sf0;     // sf0: row after row
@@ -217,8 +261,8 @@ struct Fp4CopyParams {
     int rows, src_rows, K, k_blocks, pieces;
 };
 constexpr int FP4_COPY_COLS = 1024;
-// Values from which a second kernel costs less than it saves (twice the rows of x or more; 3.7 million: 5.1 us without
-// and 6.4 us with it, 8.4 million: 7.4 and 6.6 us, 14.7 million: 11.3 and 7.4 us).  As many rows as x has: 70 us without, 82 with it.
+// Values from which a second kernel costs less than it saves (twice the rows of x or more; 3.7 million: 5 us without and 6 us
+// with it, 8.4 million: 6.5 and 6.0 us, 14.7 million: 9.5 and 6.8 us).  With as many rows as x has it loses a sixth.
 constexpr long long FP4_COPY_FROM = 1ll << 23;
 template <bool NV>
 __global__ void __launch_bounds__(FP4_QUANT_THREADS) copy_fp4_rows_kernel(const Fp4CopyParams p) {
