@@ -269,6 +269,24 @@ def test_route_equal_logits_go_to_the_lowest_index(ops):
     assert ids.cpu().tolist() == [[0, 1, 2, 3], [50, 51, 52, 53]]
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("E,n_group,topk_group", [(2, 1, 1), (8, 4, 2), (96, 1, 1), (96, 8, 3), (96, 3, 2)])
+def test_route_zeros_of_either_sign_are_equal(ops, dtype, E, n_group, topk_group):
+    """-0 and +0 have the same score: the lowest index comes first, among few keys and among more than a warp holds."""
+    logits = torch.full((4, E), -1.0)
+    logits[0, 0::2], logits[0, 1::2] = -0.0, 0.0
+    logits[1, : E // 2], logits[1, E // 2:] = -0.0, 0.0
+    logits[2, 1::4], logits[2, 3::4] = -0.0, 0.0
+    logits[3] = -0.0
+    logits = logits.to(DT[dtype])
+    k = 1 if E == 2 else 4
+    for score in ("sigmoid", "softmax"):
+        for bias in (None, torch.zeros(E), torch.full((E,), -0.0)):
+            ids, _ = ops.route(logits.cuda(), k, score=score, bias=None if bias is None else bias.cuda(), n_group=n_group, topk_group=topk_group)
+            rid, _ = _route64(logits, k, score, bias, n_group, topk_group, "top2", True, 1.0)
+            assert torch.equal(ids.cpu(), rid)
+
+
 @pytest.mark.parametrize("score", ["sigmoid", "softmax"])
 def test_route_keys_closer_than_fp32(ops, score):
     """Keys that all lie within an fp32 step of one another keep the order that 64 bits give them."""

@@ -72,8 +72,8 @@ __device__ __forceinline__ float rt_sigmoid(float x) {
     return r;
 }
 
-// PER consecutive values; -infinity behind E and for NaN.  vec: whole 16-byte pieces (E, the row distance and the base
-// allow it).
+// PER consecutive values; -infinity behind E and for NaN, +0 for -0 (equal numbers, but rt_order goes by the bits).  vec:
+// whole 16-byte pieces (E, the row distance and the base allow it).
 template <typename T, int PER>
 __device__ __forceinline__ void rt_load(const T* row, int E, int lane, bool vec, float (&l)[PER]) {
     constexpr int VL = PER < (int)(16 / sizeof(T)) ? PER : (int)(16 / sizeof(T));
@@ -91,7 +91,7 @@ __device__ __forceinline__ void rt_load(const T* row, int E, int lane, bool vec,
         for (int j = 0; j < PER; ++j) l[j] = lane * PER + j < E ? to_f32(row[lane * PER + j]) : -INFINITY;
     }
 #pragma unroll
-    for (int j = 0; j < PER; ++j) l[j] = fminf(fmaxf(l[j], -INFINITY), RT_BIG);
+    for (int j = 0; j < PER; ++j) l[j] = fminf(fmaxf(l[j] + 0.0f, -INFINITY), RT_BIG);
 }
 
 // Softmax statistics of the row: its largest logit and 1 / the sum of the exponentials (0 where every expert is off);
