@@ -300,6 +300,38 @@ def test_route_keys_closer_than_fp32(ops, score):
         assert torch.equal(ids.cpu(), rid)
 
 
+@pytest.mark.parametrize("E", [128, 256, 512, 1024])
+def test_route_one_dominating_expert(ops, E):
+    """Scores whose fp32 sum is off by a rounding per term: a bias puts another expert's key next to the dominating one's."""
+    for other in (math.log(0.51 * 2.0**-23), math.log(0.97 * 2.0**-24), -16.7, -15.544, -7.0):
+        logits = torch.full((1, E), other)
+        logits[0, 0] = 0
+        p, _ = _scores64(logits, "softmax")
+        for second in (1, E // 4, E - 1):
+            for apart in (-3e-6, -1.6e-6, -9e-7, -3e-7, 9e-8, 3e-7, 6e-7, 1.2e-6, 1.6e-6, 3e-6):
+                bias = torch.full((E,), -10.0)
+                bias[0] = 0
+                bias[second] = float(p[0, 0] - p[0, second]) - apart
+                for n_group in (1, 4):
+                    ids, _ = ops.route(logits.cuda(), 2, bias=bias.cuda(), n_group=n_group, topk_group=1, group_score="max")
+                    rid, _ = _route64(logits, 2, "softmax", bias, n_group, 1, "max", True, 1.0)
+                    assert torch.equal(ids.cpu(), rid), (other, second, apart, n_group)
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("E,n_group", [(64, 32), (96, 8), (1024, 32)])
+def test_route_groups_whose_two_best_cancel(ops, score, E, n_group):
+    """The sum of a large and a largely negative key has their rounding errors, not those of its own size."""
+    logits = _route_inputs(32, E, "fp32", 0.0, 14)
+    bias = torch.full((E,), -5000.0)
+    gs = E // n_group
+    bias[0::gs], bias[1::gs] = 1000.0, -1000.0
+    bias[: 4 * gs : gs], bias[1 : 4 * gs : gs] = 0.0, 0.0
+    ids, _ = ops.route(logits.cuda(), 4, score=score, bias=bias.cuda(), n_group=n_group, topk_group=n_group // 4)
+    rid, _ = _route64(logits, 4, score, bias, n_group, n_group // 4, "top2", True, 1.0)
+    assert torch.equal(ids.cpu(), rid)
+
+
 def test_route_extreme_logits(ops):
     big = torch.finfo(torch.float32).max
     rows = torch.tensor([[-big, -big, -big, -big], [big, 0, -big, big], [math.inf, 0, 1, 2], [-math.inf, math.nan, 5, -math.inf],

@@ -53,11 +53,20 @@ __device__ __forceinline__ uint32_t rt_order(float f) {
 __device__ __forceinline__ float rt_unorder(uint32_t o) {
     return __uint_as_float(o ^ (((int32_t)~o >> 31) | 0x80000000u));
 }
-// How far apart two fp32 keys must be for their order to be the exact one.  A score is off by less than 3e-7: sigmoid
-// p (1 - p) times the relative error of exp2 (2^-22, and |l| 2^-24 from its argument, where |l| p (1 - p) < 0.28), the
-// reciprocal 2^-23 and the addition 2^-24; softmax the like.  A bias adds half a step of the key.  The sum of a group's two
-// best doubles both.
-__device__ __forceinline__ float rt_margin(float key, bool pair) { return (pair ? 2e-6f : 1e-6f) * fmaxf(1.0f, fabsf(key)); }
+// How far apart two fp32 keys must be for their order to be the exact one: `unit` times the larger of 1 and their magnitude.
+// With u = 2^-24, an exponential's argument is off by three roundings (the difference, log2(e), the product) and exp2 by 4 u,
+// so exp(x) by (3 |x| + 4) u of itself.
+//   sigmoid   p (1 - p) (2 |l| + 4) u + 3 u p for the sum 1 + exp and the reciprocal: at most 4.5 u, as p (1 - p) |l| < 0.23;
+//             two keys, and half a step of each for the bias: 11 u.  RT_UNIT_SIGMOID is 16 u
+//   softmax   the sum of the exponentials adds PER - 1 + 5 roundings and the average of its terms' errors, (3 a + 4) u with
+//             a = sum p |x|; the reciprocal and the product two more: p (3 |x| + 3 a + PER + 14) u, where p |x| <= 1 / e and
+//             p a <= (1 - p) p ln(1023 p / (1 - p)) < 1.77.  Two keys have p + p' <= 1: (PER + 14 + 2 (3 * 1.77 + 1.11)) u, and 2 u
+//             for the bias: PER + 29.  rt_unit gives PER + 32.  (1024 experts of which one dominates: 31 u are reached)
+// A group's sum of two keys has the errors of both, by the larger one's magnitude however much of it cancels, and a rounding:
+// two groups of two such keys stay below 2 (PER + 32) u (sigmoid: 26 u).
+constexpr float RT_UNIT_SIGMOID = 16.0f / 16777216.0f;
+template <int PER> __device__ __forceinline__ float rt_unit(bool sigmoid) { return sigmoid ? RT_UNIT_SIGMOID : (PER + 32) / 16777216.0f; }
+__device__ __forceinline__ float rt_margin(float key, float unit) { return unit * fmaxf(1.0f, fabsf(key)); }
 constexpr float RT_BIG = 3.402823466e38f;           // +infinity counts as the largest number
 
 __device__ __forceinline__ float rt_ex2(float x) {
@@ -217,6 +226,7 @@ __global__ void __launch_bounds__(RT_WARPS * 32) route_kernel(const RouteParams 
     float mx = 0.0f, inv = 0.0f;
     if (!p.sigmoid) rt_softmax(l, k, &mx, &inv);
     const bool scored = p.bias != nullptr || p.n_group > 1;
+    const float unit = rt_unit<PER>(p.sigmoid);
     if (scored) {
 #pragma unroll
         for (int j = 0; j < PER; ++j) k[j] = p.sigmoid ? rt_sigmoid(l[j]) : k[j] * inv;
@@ -261,7 +271,9 @@ __global__ void __launch_bounds__(RT_WARPS * 32) route_kernel(const RouteParams 
             __syncwarp();
         }
         const int shift = even ? p.group_shift : 0, g_of = lane >> shift;          // lane g << shift has group g's score
-        const float g = p.top2 && b > -INFINITY ? a + b : a, eps = rt_margin(g, true);
+        const bool pair = p.top2 && b > -INFINITY;
+        const float g = pair ? a + b : a,
+                    eps = 2.0f * rt_margin(fmaxf(fabsf(a), pair ? fabsf(b) : 0.0f), unit);
         int before = 0, near = 0;
         for (int i = 0; i < p.n_group; ++i) {
             const float o = __shfl_sync(0xffffffffu, g, i << shift);
@@ -313,7 +325,7 @@ __global__ void __launch_bounds__(RT_WARPS * 32) route_kernel(const RouteParams 
     bound = __shfl_sync(0xffffffffu, bound, min(wanted, 32) - 1);
     if (p.bias && bound >= RT_LEAST) {              // whatever 64 bits may put among the chosen is collected too
         const float v = rt_unorder(bound);
-        bound = rt_order(v - rt_margin(v, false));
+        bound = rt_order(v - rt_margin(v, unit));
     }
     bound = max(bound, RT_LEAST);
     int count = 0;
@@ -344,7 +356,7 @@ __global__ void __launch_bounds__(RT_WARPS * 32) route_kernel(const RouteParams 
         if (p.bias) {
             const float v = rt_unorder((uint32_t)(s >> 32));
             const float next = __shfl_down_sync(0xffffffffu, v, 1);
-            if (__any_sync(0xffffffffu, lane < p.top_k && lane + 1 < total && v - next <= rt_margin(v, false))) {
+            if (__any_sync(0xffffffffu, lane < p.top_k && lane + 1 < total && v - next <= rt_margin(v, unit))) {
                 const double exact = rt_key64<T>(p, row, mine, lane);
                 rank = 0;
                 for (int i = 0; i < total; ++i) {
@@ -381,7 +393,7 @@ __global__ void __launch_bounds__(RT_WARPS * 32) route_kernel(const RouteParams 
             }
             if (p.bias) {
                 const float v = rt_unorder(m);
-                close |= last - v <= rt_margin(v, false);
+                close |= last - v <= rt_margin(v, unit);
                 last = v;
             }
         }
