@@ -332,6 +332,27 @@ def test_route_groups_whose_two_best_cancel(ops, score, E, n_group):
     assert torch.equal(ids.cpu(), rid)
 
 
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+def test_route_extreme_biases(ops, score):
+    """+infinity counts as the largest number; sums of two biases may pass the range of fp32; -infinity and NaN switch off."""
+    big, inf, off = torch.finfo(torch.float32).max, math.inf, -math.inf
+    for bias, n_group, topk_group, k in [
+            ([big, inf, 0, 0], 1, 1, 2), ([inf, big, inf, 0], 1, 1, 3), ([-big, -big, -inf, math.nan], 1, 1, 4),
+            ([inf, 1.7e38, inf, inf], 2, 1, 1), ([1.8e38, 1.7e38, 1.9e38, 1.7e38, 0, 0], 3, 1, 2), ([off, off, -big, -big], 2, 1, 2),
+            ([off, math.nan, -3e38, -2e38, -2e38, -2e38], 3, 1, 2), ([off, off, -big, off, -big, -big], 3, 2, 2), ([inf] * 96, 8, 2, 4)]:
+        b = torch.tensor(bias)
+        logits = torch.zeros((3, len(bias))).normal_(generator=gen(15))
+        logits[1] = 0
+        logits[2, :2] = off
+        ids, w = ops.route(logits.cuda(), k, score=score, bias=b.cuda(), n_group=n_group, topk_group=topk_group)
+        held = b.double().clamp(max=big)
+        gone = ~(logits > off)
+        z = torch.where(gone | ~(held > off), torch.tensor(off, dtype=torch.float64), logits.double())       # not chosen, but part of the softmax
+        rid, _ = _route64(z, k, score, torch.where(held > off, held, torch.zeros_like(held)), n_group, topk_group, "top2", True, 1.0)
+        assert torch.equal(ids.cpu(), rid), (bias, n_group)
+        assert torch.isfinite(w).all()
+
+
 def test_route_extreme_logits(ops):
     big = torch.finfo(torch.float32).max
     rows = torch.tensor([[-big, -big, -big, -big], [big, 0, -big, big], [math.inf, 0, 1, 2], [-math.inf, math.nan, 5, -math.inf],

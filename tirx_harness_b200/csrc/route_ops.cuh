@@ -42,8 +42,10 @@ struct RouteParams {
 };
 
 __device__ __forceinline__ bool rt_off(float l) { return !(l > -INFINITY); }        // -infinity or NaN
+constexpr float RT_BIG = 3.402823466e38f;           // +infinity counts as the largest number
 __device__ __forceinline__ float rt_bias(const RouteParams& p, int e) {
-    return p.bias_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[e]) : __ldg(static_cast<const float*>(p.bias) + e);
+    const float b = p.bias_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[e]) : __ldg(static_cast<const float*>(p.bias) + e);
+    return b > RT_BIG ? RT_BIG : b;                 // a NaN stays one
 }
 // larger key = larger number; 0 is below every key
 __device__ __forceinline__ uint32_t rt_order(float f) {
@@ -67,7 +69,6 @@ __device__ __forceinline__ float rt_unorder(uint32_t o) {
 constexpr float RT_UNIT_SIGMOID = 16.0f / 16777216.0f;
 template <int PER> __device__ __forceinline__ float rt_unit(bool sigmoid) { return sigmoid ? RT_UNIT_SIGMOID : (PER + 32) / 16777216.0f; }
 __device__ __forceinline__ float rt_margin(float key, float unit) { return unit * fmaxf(1.0f, fabsf(key)); }
-constexpr float RT_BIG = 3.402823466e38f;           // +infinity counts as the largest number
 
 __device__ __forceinline__ float rt_ex2(float x) {
     float r;
@@ -272,7 +273,8 @@ __global__ void __launch_bounds__(RT_WARPS * 32) route_kernel(const RouteParams 
         }
         const int shift = even ? p.group_shift : 0, g_of = lane >> shift;          // lane g << shift has group g's score
         const bool pair = p.top2 && b > -INFINITY;
-        const float g = pair ? a + b : a,
+        // a sum past the range is held at its end, next to the others there, and above a group without experts
+        const float g = pair ? fminf(fmaxf(a + b, -RT_BIG), RT_BIG) : a,
                     eps = 2.0f * rt_margin(fmaxf(fabsf(a), pair ? fabsf(b) : 0.0f), unit);
         int before = 0, near = 0;
         for (int i = 0; i < p.n_group; ++i) {
