@@ -404,6 +404,19 @@ def test_route_gradient(ops, T, E, k, dtype, score, renorm, off, pad):
     within(got, ref, allowed, "dlogits")
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_route_gradient_of_confident_sigmoids(ops, dtype):
+    """p (1 - p) keeps its relative precision where p is next to 1, and next to 0."""
+    logits = torch.cat((torch.linspace(-80, 80, 97), torch.linspace(8, 30, 63)))[None].to(DT[dtype]).repeat(5, 1)
+    ids = torch.arange(160, dtype=torch.int32).reshape(5, 32)
+    grad = torch.zeros((5, 32)).normal_(generator=gen(16))
+    got = ops.route_backward(grad.cuda(), logits.cuda(), ids.cuda(), score="sigmoid", renormalize=False)
+    z = logits.double()
+    ref = torch.zeros_like(z).scatter(1, ids.long(), grad.double() * (torch.sigmoid(z) * torch.sigmoid(-z)).gather(1, ids.long()))
+    # p and 1 - p: an exponential of 2 steps (4 roundings), a sum and a division each; then three products
+    within(got, ref, (half_step(DT[dtype]) + 16 * U32) * ref.abs() + torch.finfo(DT[dtype]).tiny, "dlogits")
+
+
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("renorm", [True, False])
 def test_route_gradient_against_differences(ops, score, renorm):

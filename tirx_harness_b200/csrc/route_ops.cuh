@@ -460,7 +460,7 @@ __global__ void __launch_bounds__(RT_WARPS * 32) route_grad_kernel(const RouteGr
         g = id >= 0 ? __fdiv_rn(g - __fdiv_rn(dot, total), total) : 0.0f;
     }
     float c = g * s, minus = 0.0f;
-    if (p.sigmoid) c *= 1.0f - s;
+    if (p.sigmoid) c *= __fdiv_rn(1.0f, 1.0f + expf(li));          // 1 - s, which loses its bits as s nears 1
     else {
         minus = -warp_sum(c);
 #pragma unroll
