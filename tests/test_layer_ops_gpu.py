@@ -404,6 +404,70 @@ def test_route_gradient(ops, T, E, k, dtype, score, renorm, off, pad):
     within(got, ref, allowed, "dlogits")
 
 
+def _route_grad64_of_differences(grad, logits, ids, score, renorm):
+    """The same without differences of nearly equal scores, and the sum of the magnitudes of its terms."""
+    p, _ = _scores64(logits, score)
+    T, E = p.shape
+    out, mag = torch.zeros_like(p), torch.zeros_like(p)
+    for t in range(T):
+        at = [int(i) for i in ids[t] if i >= 0]
+        G = torch.tensor([float(grad[t, j]) for j in range(ids.shape[1]) if ids[t, j] >= 0], dtype=torch.float64)
+        s = p[t, at]
+        rest = 1.0 if score == "sigmoid" else float(p[t, [e for e in range(E) if e not in at]].sum())
+        total = float(s.sum()) + 1e-20
+        d = (G[:, None] - G[None]) * s[None]
+        if renorm:
+            h, hm = (d.sum(1) + 1e-20 * G) / total**2, (d.abs().sum(1) + 1e-20 * G.abs()) / total**2
+            others = float((G * s).sum()) * 1e-20 / total**2
+        elif score == "softmax":
+            h, hm, others = d.sum(1) + G * rest, d.abs().sum(1) + G.abs() * rest, float((G * s).sum())
+        else:
+            h, hm = G, G.abs()
+        if score == "sigmoid":
+            f = torch.sigmoid(-logits[t, at].double())
+            once, oncem = s * f * h, s * f * hm
+        else:
+            once = s * (h - (others if renorm else 0))
+            oncem = s * (hm + (abs(others) if renorm else 0))
+            out[t], mag[t] = -p[t] * others, p[t] * float((G * s).abs().sum()) * (1e-20 / total**2 if renorm else 1)
+            out[t, at], mag[t, at] = 0, 0
+        for j, e in enumerate(at):
+            out[t, e] += once[j]
+            mag[t, e] += oncem[j]
+    return out, mag
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renorm", [True, False])
+@pytest.mark.parametrize("dtype,E,k", [("fp32", 64, 8), ("bf16", 256, 3), ("fp32", 1000, 32), ("fp32", 6, 1)])
+def test_route_gradient_where_one_score_dominates(ops, score, renorm, dtype, E, k):
+    """Relative to the terms that are left once p next to 1 is not subtracted from 1."""
+    logits = _route_inputs(12, E, "fp32", 0.0, 17) * 0.5
+    for t in range(12):
+        logits[t, (5 * t) % E] = 2.5 * t
+    logits = logits.to(DT[dtype])
+    grad = torch.zeros((12, k)).normal_(generator=gen(18))
+    grad[1] = 0.75                                     # equal gradients: nothing left where they are renormalised
+    ids, _ = _route64(logits, k, score, None, 1, 1, "max", renorm, 1.0)
+    if k > 2:
+        ids[2, 1], ids[3, 0] = -1, ids[3, 2]           # the same index twice counts twice
+        twice = ids[3].clone()
+    got = ops.route_backward(grad.cuda(), logits.cuda(), ids.cuda(), score=score, renormalize=renorm)
+    rows = [t for t in range(12) if t != 3]            # a row with an index twice: against the plain form below
+    ref, mag = _route_grad64_of_differences(grad[rows], logits[rows], ids[rows], score, renorm)
+    plain = _route_grad64(grad[rows], logits[rows], ids[rows], score, renorm, 1.0)
+    assert ((ref - plain).abs() <= 1e-12 * (1 + plain.abs())).all()
+    # a score: 4 roundings of its exponential and as many as its argument's size (at most 30, from three roundings each), the sum
+    # of up to 32 in a lane and five levels, and a division; four scores, k products and a few more steps
+    allowed = 4 * (4 + 3 * 30 + 40) + k + 10
+    within(got[rows], ref, half_step(logits.dtype) * ref.abs() + allowed * U32 * mag + torch.finfo(logits.dtype).tiny, "dlogits")
+    if k > 2:
+        plain = _route_grad64(grad[3:4], logits[3:4], twice[None], score, renorm, 1.0)
+        p, _ = _scores64(logits[3:4], score)
+        total = p.gather(1, twice[None].long()).sum() if renorm else 1
+        within(got[3:4], plain, half_step(logits.dtype) * plain.abs() + 256 * U32 * p * k * grad[3].abs().max() * (2 / total if renorm else 1), "twice")
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 def test_route_gradient_of_confident_sigmoids(ops, dtype):
     """p (1 - p) keeps its relative precision where p is next to 1, and next to 0."""
