@@ -240,7 +240,9 @@ int moe_combine(const void* y_bf16, const int32_t* pos, const float* w, void* ou
  * weight [H] of w_dtype (dtype or f32).  residual may be NULL (then h is x, and h is not written).  h and y (may be NULL:
  * the unquantised output) are dense [T, H] of `dtype`; q dense e4m3 [T, H]; scales at [r * ss_row + block * ss_blk];
  * rstd f32 [T].  H % 8 == 0, H <= 16384; pointers 16-byte aligned.  Sums are kept in fp32.  h and y may not overlap the inputs.
- * A row with a NaN or an infinity has NaN in its scales and codes.  The reference has no counterpart. */
+ * A NaN in a row makes all its scales and codes NaN.  An infinity in h makes rstd 0: its own 128 columns get the scale NaN, the
+ * others zeros under the smallest scale.  Finite rows are normalised whatever their size, also where h^2 passes fp32's range.
+ * The reference has no counterpart. */
 typedef struct moe_norm_args {
     const void* x;
     int64_t x_stride;

@@ -142,6 +142,38 @@ def test_norm_zero_rows_nan_and_infinity(ops):
     assert empty["q"].shape == (0, 256) and empty["scales"].shape == (0, 2)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("H", [256, 1000, 7168, 16384])
+@pytest.mark.parametrize("residual", [False, True])
+def test_norm_rows_whose_squares_pass_the_range(ops, dtype, H, residual):
+    """Finite rows of any size are normalised; one with an infinity shows it in its own block and is zero elsewhere."""
+    size = [1e18, 2e19, 1.0, 1e25, 5e30, 8e36, 3e38, 1e22]
+    x = torch.zeros((8, H)).normal_(generator=gen(6)).clamp(-1, 1) * torch.tensor(size)[:, None]
+    x[6] = 3.3e38 * torch.sign(x[6])
+    x[7, H // 2] = math.inf
+    x = x.to(DT[dtype])
+    r = torch.zeros_like(x) if residual else None
+    w = 1 + 0.2 * torch.zeros(H).normal_(generator=gen(7))
+    got = ops.rms_norm_quant(x.cuda(), w.cuda(), residual=r.cuda() if residual else None, want_y=True)
+    h = x.double()[:7]
+    rstd = (h.square().mean(1) + 1e-6).rsqrt()
+    e = 50 * U32                               # as above
+    within(got["rstd"][:7], rstd, e * rstd + 2.0**-149, "rstd")
+    y = h * rstd[:, None] * w.double()
+    within(got["y"][:7], y, (half_step(x.dtype) + e + 2 * U32) * y.abs() + torch.finfo(x.dtype).tiny, "y")
+    nb = (H + 127) // 128
+    s = torch.nn.functional.pad(y, (0, nb * 128 - H)).reshape(7, nb, 128).abs().amax(2).clamp(min=1e-8) / 448
+    within(got["scales"][:7], s, (e + 4 * U32) * s, "scales")
+    t = y / got["scales"][:7].cpu().double().repeat_interleave(128, 1)[:, :H]
+    step = torch.maximum(t.abs() * 2.0**-4, torch.tensor(2.0**-10, dtype=torch.float64))
+    within(got["q"][:7].float(), t, step + 2 * e * t.abs(), "q")
+    own = H // 2 // 128
+    scales, codes = got["scales"][7].cpu(), got["q"][7].float().cpu()
+    assert torch.isnan(scales[own]) and torch.isnan(codes[own * 128 : (own + 1) * 128]).all()
+    rest = torch.arange(nb) != own
+    assert (scales[rest] == np.float32(1e-8) / np.float32(448)).all() and (codes[rest.repeat_interleave(128)[:H]] == 0).all()
+
+
 @pytest.mark.parametrize("T,H,dtype,w32,dh", [(1, 7168, "bf16", False, True), (3, 8, "fp32", True, False), (517, 1000, "fp16", True, True),
                                               (700, 2048, "fp32", False, False), (300, 7168, "bf16", True, True), (5, 12296, "fp32", False, True),
                                               (6, 16384, "bf16", False, False)])

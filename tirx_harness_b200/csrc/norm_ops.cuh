@@ -35,7 +35,7 @@ struct NormParams {
 constexpr int NORM_MAX_THREADS = 512;
 constexpr int NORM_MAX_H = 512 * 4 * 8;        // four pieces of 8 columns per thread
 constexpr int NORM_MAX_STAGES = 4;
-constexpr int NORM_HEAD_BYTES = 512;           // shared memory in front of the ring: barriers, sums, flags
+constexpr int NORM_HEAD_BYTES = 512;           // shared memory in front of the ring: barriers, flags, from 128 on the sums
 
 // The ring of rows: `streams` inputs of `row_bytes` each per stage.  Thread 0 issues, everybody waits.
 struct RowRing {
@@ -79,12 +79,82 @@ __device__ __forceinline__ float block_sum(float v, float* buf) {
     return warp_sum(lane < warps ? buf[lane] : 0.0f);          // every warp for itself, in the same order
 }
 
+// Piece i of row `row` of y: the scale of its 128 columns from its largest magnitude, and y, scale and codes are stored.  All threads
+// of a warp take part; pieces from H / 8 on have amax 0 and are not stored.
+template <typename T>
+__device__ __forceinline__ void norm_put(const NormParams& p, int row, int i, float amax, f32x2 (&y)[4]) {
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) amax = amax_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    if (i < (p.H >> 3)) {
+        float s = __fdiv_rn(amax < 1.0e-8f ? 1.0e-8f : amax, 448.0f);          // a NaN stays one
+        if (p.pow2 && s < INFINITY) s = __uint_as_float((__float_as_uint(s) + 0x7FFFFFu) & 0xFF800000u);     // up to the next power of two
+        if ((i & 15) == 0) p.scales[row * p.ss_row + (i >> 4) * p.ss_blk] = s;
+        if (p.y) store8(static_cast<T*>(p.y) + (long long)row * p.H + i * 8, pack8<T>(y));
+        div8(y, s);
+        *reinterpret_cast<uint2*>(p.q + (long long)row * p.H + i * 8) = pack8_e4m3(y);
+    }
+}
+
+// The rows of this block whose squares pass fp32's range (rstd is 0) once more, in units of 2^72; a row with an infinity comes out
+// as it was.  Called by the whole block behind its loop, whose registers and time it leaves alone (16384 x 7168: 130 us; inside the
+// loop 137 us).
+template <typename T, typename W>
+__device__ __noinline__ void rms_norm_again(const NormParams p, float* sums) {
+    constexpr float unit = 0x1p-72f;
+    const int n8 = p.H >> 3, step = gridDim.x;
+    auto load = [&](int row, int i, f32x2 (&h)[4]) {
+        unpack8(load8(static_cast<const T*>(p.x) + row * p.x_stride + i * 8), h);
+        if (!p.residual) return;
+        f32x2 r[4];
+        unpack8(load8(static_cast<const T*>(p.residual) + row * p.res_stride + i * 8), r);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) h[j] = add2(h[j], r[j]);
+        unpack8(pack8<T>(h), h);
+    };
+    __syncthreads();
+    for (int row = blockIdx.x;; row += step) {
+        if (*static_cast<volatile const float*>(p.rstd + row) == 0.0f) {          // the same for all threads
+            f32x2 sq = 0, h[4];
+            for (int i = threadIdx.x; i < n8; i += blockDim.x) {
+                load(row, i, h);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    h[j] = mul2(h[j], both(unit));
+                    sq = fma2(h[j], h[j], sq);
+                }
+            }
+            const float total = block_sum(lo2(sq) + hi2(sq), sums);
+            const float rstd = __frsqrt_rn(__fdiv_rn(total, (float)p.H) + p.eps * unit * unit) * unit;
+            if (threadIdx.x == 0) p.rstd[row] = rstd;
+            for (int base = 0; base < n8; base += blockDim.x) {
+                const int i = base + threadIdx.x;
+                float amax = 0.0f;
+                if (i < n8) {
+                    f32x2 w[4];
+                    load(row, i, h);
+                    unpack8(load8(static_cast<const W*>(p.weight) + i * 8), w);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        h[j] = mul2(mul2(h[j], both(rstd)), w[j]);
+                        amax = amax_nan(amax_nan(amax, lo2(h[j])), hi2(h[j]));
+                    }
+                }
+                norm_put<T>(p, row, i, amax, h);
+            }
+            __syncthreads();                   // the sums have been read
+        }
+        if (p.T - row <= step) break;
+    }
+}
+
 // Thread t holds the 8-column pieces t, t + blockDim, ... (CH of them).  A 128-column block is 16 neighbouring threads of
 // one piece, so its largest value takes four shuffles.
 template <typename T, typename W, int CH>
 __global__ void __launch_bounds__(NORM_MAX_THREADS) rms_norm_quant_kernel(const NormParams p) {
     extern __shared__ __align__(128) uint8_t smem[];
     float* sums = reinterpret_cast<float*>(smem + 128);
+    volatile int* past = reinterpret_cast<volatile int*>(smem + 96);          // a sum of squares was infinite
+    if (threadIdx.x == 0) *past = 0;
     const int n8 = p.H >> 3, step = gridDim.x;
     const bool res = p.residual != nullptr;
     RowRing ring(smem, p.stages, p.H * (int)sizeof(T), res ? 2 : 1, p.status);
@@ -132,7 +202,10 @@ __global__ void __launch_bounds__(NORM_MAX_THREADS) rms_norm_quant_kernel(const 
         if (threadIdx.x == 0 && ahead < p.T) fetch(ring.stage, (int)ahead);
         ring.next();
         const float rstd = __frsqrt_rn(__fdiv_rn(total, (float)p.H) + p.eps);
-        if (threadIdx.x == 0) p.rstd[row] = rstd;
+        if (threadIdx.x == 0) {
+            p.rstd[row] = rstd;
+            if (rstd == 0.0f) *past = 1;
+        }
         const f32x2 rstd2 = both(rstd);
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
@@ -145,20 +218,13 @@ __global__ void __launch_bounds__(NORM_MAX_THREADS) rms_norm_quant_kernel(const 
                 h[c][j] = i < n8 ? mul2(mul2(h[c][j], rstd2), w[j]) : 0;
                 amax = amax_nan(amax_nan(amax, lo2(h[c][j])), hi2(h[c][j]));
             }
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) amax = amax_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-            if (i < n8) {
-                float s = __fdiv_rn(amax < 1.0e-8f ? 1.0e-8f : amax, 448.0f);          // a NaN stays one
-                if (p.pow2 && s < INFINITY) s = __uint_as_float((__float_as_uint(s) + 0x7FFFFFu) & 0xFF800000u);     // up to the next power of two
-                if ((i & 15) == 0) p.scales[row * p.ss_row + (i >> 4) * p.ss_blk] = s;
-                if (p.y) store8(static_cast<T*>(p.y) + (long long)row * p.H + i * 8, pack8<T>(h[c]));
-                div8(h[c], s);
-                *reinterpret_cast<uint2*>(p.q + (long long)row * p.H + i * 8) = pack8_e4m3(h[c]);
-            }
+            norm_put<T>(p, row, i, amax, h[c]);
         }
         if (p.T - row <= step) break;          // row + step could pass 2^31
         row += step;
     }
+    __syncthreads();
+    if (*past) rms_norm_again<T, W>(p, sums);
 }
 
 struct NormGradParams {
