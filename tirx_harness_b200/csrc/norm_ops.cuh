@@ -46,6 +46,7 @@ struct RowRing {
     int stages, row_bytes, streams;
     int stage = 0;
     uint32_t phase = 0;
+    bool live = true;
 
     __device__ __forceinline__ RowRing(uint8_t* smem, int stages_, int row_bytes_, int streams_, int* status_)
         : full(reinterpret_cast<uint64_t*>(smem)), data(smem + NORM_HEAD_BYTES),
@@ -65,8 +66,15 @@ struct RowRing {
     __device__ __forceinline__ void load_once(int s, int stream, const void* src) const {
         bulk_load_once(smem_u32(at(s, stream)), src, row_bytes, smem_u32(full + s));
     }
-    // A wait that runs out sets the status word; the row is then made of whatever the stage holds.
-    __device__ __forceinline__ void wait() const { mbar_wait_warp(smem_u32(full + stage), phase, abort_flag, status, STATUS_TIMEOUT_SMEM_FULL); }
+    // A wait that runs out sets the status word; this row and those behind it are then made of whatever the stages hold, thread 0
+    // issues no further copies, and those in flight get time to land before the block's memory goes (leave).
+    __device__ __forceinline__ void wait() { live = mbar_wait_warp(smem_u32(full + stage), phase, abort_flag, status, STATUS_TIMEOUT_SMEM_FULL) && live; }
+    __device__ __forceinline__ void leave() const {
+        if (threadIdx.x == 0 && !live) {
+            const uint64_t t0 = globaltimer_ns();
+            while (globaltimer_ns() - t0 < 1000000ull) {}
+        }
+    }
     __device__ __forceinline__ void next() { if (++stage == stages) { stage = 0; phase ^= 1; } }
 };
 
@@ -199,7 +207,7 @@ __global__ void __launch_bounds__(NORM_MAX_THREADS) rms_norm_quant_kernel(const 
         const float total = block_sum(lo2(sq) + hi2(sq), sums + flip);
         // the stage has been read by every thread: it can take the row after those under way
         const long long ahead = (long long)row + (long long)p.stages * step;
-        if (threadIdx.x == 0 && ahead < p.T) fetch(ring.stage, (int)ahead);
+        if (threadIdx.x == 0 && ring.live && ahead < p.T) fetch(ring.stage, (int)ahead);
         ring.next();
         const float rstd = __frsqrt_rn(__fdiv_rn(total, (float)p.H) + p.eps);
         if (threadIdx.x == 0) {
@@ -223,6 +231,7 @@ __global__ void __launch_bounds__(NORM_MAX_THREADS) rms_norm_quant_kernel(const 
         if (p.T - row <= step) break;          // row + step could pass 2^31
         row += step;
     }
+    ring.leave();
     __syncthreads();
     if (*past) rms_norm_again<T, W>(p, sums);
 }
@@ -295,7 +304,7 @@ __global__ void __launch_bounds__(NORM_MAX_THREADS) rms_norm_grad_kernel(const N
         }
         const float mean = __fdiv_rn(block_sum(lo2(dot) + hi2(dot), sums + flip), (float)p.H);
         const long long ahead = (long long)row + (long long)p.stages * step;
-        if (threadIdx.x == 0 && ahead < p.T) fetch(ring.stage, (int)ahead);
+        if (threadIdx.x == 0 && ring.live && ahead < p.T) fetch(ring.stage, (int)ahead);
         ring.next();
         const f32x2 minus_mean = both(-mean);
 #pragma unroll
@@ -319,6 +328,7 @@ __global__ void __launch_bounds__(NORM_MAX_THREADS) rms_norm_grad_kernel(const N
         if (p.T - row <= step) break;
         row += step;
     }
+    ring.leave();
     pdl_launch_dependents();                   // the kernel that adds the shares up may be scheduled; it waits for this one's end
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
