@@ -130,6 +130,20 @@ def test_tensors_on_the_host_are_refused():
         moe_ops.route(x.long(), 2)
 
 
+@pytest.mark.parametrize("at,value,error,word", [
+    ("T", 1 << 31, ValueError, "T=2147483648"), ("stride", 1 << 63, ValueError, "stride="), ("n_group", 2.0, TypeError, "n_group"),
+    ("topk_group", "2", TypeError, "topk_group"), ("scale", None, TypeError, "scale"), ("scale", 10**400, ValueError, "scale=")])
+def test_values_that_do_not_fit_are_refused_by_name(lib, at, value, error, word):
+    """Before any CUDA call, and as the other checks of arguments refuse."""
+    from tirx_harness_b200 import moe_ops
+    block = dict(logits=A16, stride=64, bias=0, ids=A16, weights=A16, T=4, E=64, top_k=2, n_group=1, topk_group=1, dtype=0, bias_dtype=0,
+                 score=0, group_score=0, renormalize=1, scale=1.0)
+    assert list(block) == [f[0] for f in lib.RouteArgs._fields_]
+    block[at] = value
+    with pytest.raises(error, match=word):
+        moe_ops._launch(lib.ROUTE, torch.device("cuda", 0), *block.values())
+
+
 def test_scale_tile_shapes():
     from tirx_harness_b200 import moe_ops
     assert moe_ops.fp4_scale_shape(1, 128, "nvfp4") == (1, 4, 512)

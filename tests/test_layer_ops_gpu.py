@@ -1059,6 +1059,21 @@ def test_refusals(ops, gg):
             pytest.fail(f"call {i} is not refused")
 
 
+def test_arguments_of_another_kind_are_refused(ops):
+    logits = torch.zeros((2, 16), device="cuda")
+    for kw in (dict(n_group=2.0), dict(topk_group="1"), dict(scale=None)):
+        with pytest.raises(TypeError):
+            ops.route(logits, 2, **kw)
+    for kw in (dict(n_group=1 << 40), dict(scale=10**400)):
+        with pytest.raises(ValueError):
+            ops.route(logits, 2, **kw)
+    with pytest.raises(TypeError):
+        ops.rms_norm_quant(torch.zeros((2, 128), device="cuda"), torch.ones(128, device="cuda"), eps="1e-6")
+    with pytest.raises(TypeError):
+        ops.quant_fp4(torch.zeros((2, 128), device="cuda"), src_pair=torch.zeros(2, dtype=torch.int32, device="cuda"), top_k=1.5)
+
+
+
 # ------------------------------------------------------------------ offsets past 32 bits
 def test_offsets_past_32_bits(ops, gg):
     """More than 2^32 bytes (and 2^31 elements) in front of the last rows, which are compared with the same rows alone."""

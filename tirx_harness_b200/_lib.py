@@ -230,7 +230,20 @@ class Entry:
     def __init__(self, name: str, args):
         layout = struct.Struct("@" + "".join(self._CODES[t] for _, t in args._fields_) + "0P")
         assert layout.size == _c.sizeof(args), name
-        self.pack, self._name, self._fn = layout.pack, name, None
+        self.pack, self._name, self._fn, self._fields = layout.pack, name, None, args._fields_
+
+    def misfit(self, values) -> Exception:
+        """What is wrong with values that ``pack`` could not lay out."""
+        for (field, kind), v in zip(self._fields, values):
+            try:
+                struct.pack("@" + self._CODES[kind], v)
+            except OverflowError:
+                return ValueError(f"{field}={v} does not fit its {_c.sizeof(kind) * 8} bits")
+            except struct.error:
+                if hasattr(v, "__index__"):
+                    return ValueError(f"{field}={v} does not fit its {_c.sizeof(kind) * 8} bits")
+                return TypeError(f"{field} must be {'a number' if kind is _c.c_float else 'an integer'}, got {v!r}")
+        return TypeError(f"{self._name} takes {len(self._fields)} values, got {len(values)}")
 
     def _bind(self):
         self._fn = _c.CFUNCTYPE(_c.c_int, *self._ARGTYPES)((self._name, lib()))

@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
@@ -176,12 +177,16 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda in
 
 def _launch(entry, device, *values):
     """Calls an entry point on the current stream of the tensors' device, which need not be the current one."""
+    try:
+        block = entry.pack(*values)
+    except (struct.error, OverflowError):
+        raise entry.misfit(values) from None
     index = device.index
     if index == torch.cuda.current_device():
-        entry(entry.pack(*values), _raw_stream(index))
+        entry(block, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            entry(entry.pack(*values), _raw_stream(index))
+            entry(block, _raw_stream(index))
 
 
 def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-6,
