@@ -101,6 +101,20 @@ def test_product_refuses(lib, fn, kw, word):
     _refused(lib, fn, lib.GGFp4Args(**(base | kw)), word)
 
 
+def test_row_counts_at_the_end_of_32_bits_are_refused(lib):
+    """Rounded up to whole blocks they would pass 2^31."""
+    top = (1 << 31) - 1
+    for T in (top, top - 126):
+        _refused(lib, "moe_route", lib.RouteArgs(**(ROUTE | dict(T=T))), "T=")
+        _refused(lib, "moe_route_backward", lib.RouteGradArgs(grad_weights=A16, logits=A16, stride=64, ids=A16, dlogits=A16, T=T, E=64, top_k=8, dtype=1), "T=")
+        quant = dict(x=A16, x_stride=256, src_pair=A16, q=A16, scales=A16, groups=1, rows=T, src_rows=4, K=128, top_k=1, gate_first=1)
+        _refused(lib, "moe_quant_fp4", lib.Fp4QuantArgs(**quant), "rows=")
+        product = dict(a=A16, sfa=A16, b=A16, sfb=A16, layout=A16, d=A16, ldd=64, G=1, M=T, N=64, K=128)
+        for fn in ("moe_gg_fp4_contiguous", "moe_gg_fp4_masked"):
+            _refused(lib, fn, lib.GGFp4Args(**product), "scales")
+            _refused(lib, fn, lib.GGFp4Args(**(product | dict(M=4, N=top - 7, ldd=top - 7))), "scales")
+
+
 def test_unpack_refuses(lib):
     f = lib.lib().moe_unpack_fp4
     p = ctypes.c_void_p

@@ -6,6 +6,8 @@ namespace {
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 inline bool float_dtype(int d) { return d == MOE_DTYPE_BF16 || d == MOE_DTYPE_F32 || d == MOE_DTYPE_F16; }
+// Most rows of a call whose kernels count rows and blocks of up to 128 of them in 32 bits.
+constexpr int32_t MAX_ROWS_32 = 0x7FFFFFFF - 127;
 inline int dtype_bytes(int d) { return d == MOE_DTYPE_F32 ? 4 : 2; }
 
 // f(a value of the element type)
@@ -114,7 +116,8 @@ int launch_norm_grad(const NormGradParams& p, float* dw, NormShape s, DeviceInfo
 }
 
 int check_route(int32_t T, int32_t E, int32_t top_k, int32_t dtype, int32_t score, int64_t stride) {
-    if (T < 0 || E <= 0 || E > RT_MAX_E) return fail(MOE_ERR_INVALID, "T=%d must be non-negative and E=%d in [1, %d]", T, E, RT_MAX_E);
+    if (T < 0 || T > MAX_ROWS_32 || E <= 0 || E > RT_MAX_E)
+        return fail(MOE_ERR_INVALID, "T=%d must be in [0, %d] and E=%d in [1, %d]", T, MAX_ROWS_32, E, RT_MAX_E);
     if (top_k <= 0 || top_k > 32 || top_k > E) return fail(MOE_ERR_INVALID, "top_k=%d must be in [1, min(32, E)]", top_k);
     if (!float_dtype(dtype)) return fail(MOE_ERR_INVALID, "dtype must be bf16, f16 or f32");
     if (score != MOE_SCORE_SOFTMAX && score != MOE_SCORE_SIGMOID) return fail(MOE_ERR_INVALID, "score must be MOE_SCORE_SOFTMAX or MOE_SCORE_SIGMOID");
@@ -245,8 +248,8 @@ int launch_gg_fp4(const moe_gg_fp4_args* a, bool masked, void* stream) {
     if (masked && a->G > gg::MAX_MASKED_GROUPS) return fail(MOE_ERR_INVALID, "masked layout supports at most %d groups", gg::MAX_MASKED_GROUPS);
     const long long rows_total = masked ? (long long)a->G * a->M : (long long)a->M;
     if (rows_total > 0x7FFFFFFFll || (long long)a->G * a->N > 0x7FFFFFFFll) return fail(MOE_ERR_INVALID, "row counts exceed 2^31-1");
-    const long long chunks = (masked ? (long long)a->G : 1) * ((a->M + 127) / 128) + (long long)a->G * ((a->N + 127) / 128);
-    if (chunks * ((a->K + 255) / 256) > 0x7FFFFFFFll / 256) return fail(MOE_ERR_INVALID, "the scales exceed 2^31 64-bit words");
+    const long long chunks = (masked ? (long long)a->G : 1) * ((a->M + 127ll) / 128) + (long long)a->G * ((a->N + 127ll) / 128);
+    if (chunks * ((a->K + 255ll) / 256) > 0x7FFFFFFFll / 256) return fail(MOE_ERR_INVALID, "the scales exceed 2^31 64-bit words");
     if (a->alpha && a->alpha_stride != 0 && a->alpha_stride != 1) return fail(MOE_ERR_INVALID, "alpha_stride must be 0 or 1");
     if (rows_total == 0) return MOE_OK;
     if (!a->a || !a->sfa || !a->b || !a->sfb || !a->layout || !a->d) return fail(MOE_ERR_INVALID, "a, sfa, b, sfb, layout and d must all be non-NULL");
@@ -390,8 +393,8 @@ size_t moe_quant_fp4_workspace_bytes(int32_t rows, int32_t src_rows, int32_t K, 
 
 int moe_quant_fp4(const moe_fp4_quant_args* a, void* stream) {
     if (!a) return fail(MOE_ERR_INVALID, "args is NULL");
-    if (a->groups <= 0 || a->groups > 65535 || a->rows < 0 || a->src_rows < 0 || a->K <= 0 || a->K % 128)
-        return fail(MOE_ERR_INVALID, "groups must be in [1, 65535], rows non-negative and K=%d a positive multiple of 128", a->K);
+    if (a->groups <= 0 || a->groups > 65535 || a->rows < 0 || a->rows > MAX_ROWS_32 || a->src_rows < 0 || a->K <= 0 || a->K % 128)
+        return fail(MOE_ERR_INVALID, "groups must be in [1, 65535], rows=%d in [0, %d] and K=%d a positive multiple of 128", a->rows, MAX_ROWS_32, a->K);
     if (a->format != MOE_FP4_NV && a->format != MOE_FP4_MX) return fail(MOE_ERR_INVALID, "format must be MOE_FP4_NV or MOE_FP4_MX");
     if (!float_dtype(a->dtype)) return fail(MOE_ERR_INVALID, "dtype must be bf16, f16 or f32");
     if (a->src_pair ? a->groups != 1 || a->top_k <= 0 : a->rows != a->src_rows)
