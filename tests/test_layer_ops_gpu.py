@@ -1059,6 +1059,16 @@ def test_refusals(ops, gg):
             pytest.fail(f"call {i} is not refused")
 
 
+def test_product_refuses_an_empty_rows_used(ops, gg):
+    """Its address is NULL, which means that all rows are in use."""
+    a, sfa = ops.quant_fp4(torch.zeros((4, 256), device="cuda"))
+    b, sfb = ops.quant_fp4(torch.zeros((2, 64, 256), device="cuda"))
+    d, lay = torch.zeros((4, 64), device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda")
+    gg.bind_contiguous_fp4(a, sfa, b, sfb, d, lay, rows_used=lay[:1])
+    with pytest.raises(ValueError):
+        gg.bind_contiguous_fp4(a, sfa, b, sfb, d, lay, rows_used=lay[:0])
+
+
 def test_arguments_of_another_kind_are_refused(ops):
     logits = torch.zeros((2, 16), device="cuda")
     for kw in (dict(n_group=2.0), dict(topk_group="1"), dict(scale=None)):

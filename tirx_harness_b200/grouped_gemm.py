@@ -287,8 +287,8 @@ def bind_contiguous_fp4(a, sfa, b, sfb, d, grouped_layout, alpha=None, fmt: str 
         raise ValueError(f"d must be bfloat16 (or float32) [{M}, {N}] with unit column stride on {b.device}")
     if grouped_layout.numel() != M:
         raise ValueError(f"grouped_layout must be int32 [{M}]")
-    if rows_used is not None and (rows_used.dtype != torch.int32 or rows_used.device != b.device):
-        raise ValueError(f"rows_used must be an int32 tensor on {b.device}")
+    if rows_used is not None and (rows_used.dtype != torch.int32 or rows_used.device != b.device or rows_used.numel() == 0):
+        raise ValueError(f"rows_used must be an int32 [1] tensor on {b.device}")
     return _BoundFp4(_lib.GG_FP4_CONTIGUOUS, a, sfa, b, sfb, d, grouped_layout, alpha, fmt, G, M, N, K, rows_used)
 
 
