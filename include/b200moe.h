@@ -324,7 +324,8 @@ int moe_route_backward(const moe_route_grad_args* args, void* stream);
 /* 4-bit block formats.  Codes are e2m1 (0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives), two to a byte, the earlier
  * in the low half.
  *   MOE_FP4_NV  one e4m3 scale s per 16 values and one fp32 factor g: value = code * s * g; quantisation takes
- *               s = e4m3(min(amax / (6 g), 448)), code = e2m1(x / (s g))
+ *               s = e4m3(min(amax / (6 g), 448)), code = e2m1(x / (s g)).  g = largest magnitude / (6 * 448) uses the
+ *               scales' whole range; a block whose largest magnitude is at most 6 * 2^-10 g becomes zero
  *   MOE_FP4_MX  one UE8M0 scale per 32 values: s = 2^(floor(log2 amax) - 2), at least 2^-127; code = e2m1(x / s)
  * (round to nearest even; magnitudes above 6 become 6).  A block that holds an infinity or a NaN gets the scale NaN.
  * Scales lie in tiles of 512 bytes for 128 rows x 4 blocks: uint8 [row blocks of 128][ceil(K/256) * (4 NV, 2 MX)][512],

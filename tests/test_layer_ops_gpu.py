@@ -925,6 +925,36 @@ def _layer(ops, gg, x, res, wn, wr, bias, w13, w2, top_k, work):
     return dict(n=n, ids=ids, w=w, plan=plan, a1=a1, a2=a2, out=ops.combine(work["y"], plan["pos"], w))
 
 
+def test_product_of_quantised_weights_is_near_the_product_of_the_weights(ops, gg):
+    """With g = largest magnitude / (6 * 448) no block of ordinary weights vanishes, and the product keeps to the format's steps."""
+    E, N, K, rows = 3, 264, 1408, 150
+    w = torch.zeros((E, N, K)).normal_(generator=gen(71)) / K**0.5 * torch.tensor([1.0, 0.05, 20.0])[:, None, None]
+    x = torch.zeros((rows, K)).normal_(generator=gen(72))
+    layout = torch.arange(rows, dtype=torch.int32) * E // rows
+    gw, gx = w.abs().amax((1, 2)) / (6 * 448), x.abs().amax().reshape(1) / (6 * 448)
+    qw, qx = ops.quant_fp4(w.cuda(), global_scale=gw.cuda()), ops.quant_fp4(x.cuda(), global_scale=gx.cuda())
+    d = torch.zeros((rows, N), device="cuda")
+    gg.bind_contiguous_fp4(*qx, *qw, d, layout.cuda(), alpha=(gx * gw).cuda())()
+
+    def step(v):                               # of each value: the largest error of its block
+        amax = v.double().reshape(*v.shape[:-1], -1, 16).abs().amax(-1)
+        # scales of normal e4m3 numbers (half a step: 2^-4); then the codes' largest half step is 1 in units of the scale, amax / 6
+        assert (amax > v.double().abs().amax((-2, -1), keepdim=True) * 2.0**-6 / 448).all()
+        return ((1 + 2.0**-4 + 1e-6) / 6 * amax).repeat_interleave(16, -1)
+    sw, sx = step(w), step(x)
+    back = torch.stack([torch.from_numpy(E2M1[codes_of(qw[0][e])] * np.repeat(scale_values(scale_bytes(qw[1][e], N, K, "nvfp4"), "nvfp4"), 16, -1)) * float(gw[e])
+                        for e in range(E)])
+    assert ((back - w.double()).abs() <= sw).all()
+    for e in range(E):
+        at = (layout == e).nonzero().flatten()
+        ref = x[at].double() @ w[e].double().T
+        off = sx[at] @ w[e].double().abs().T + x[at].double().abs() @ sw[e].T + sx[at] @ sw[e].T
+        # (fp32 sums: K 2^-24 of the sum of magnitudes, of which `off` is a third and more)
+        within(d[at.cuda()], ref, off * (1 + 1e-3), "product")
+        # errors of random signs grow with the root of K: a sixth of the sum of the bounds is far above them
+        assert (d[at.cuda()].cpu().double() - ref).norm() < off.norm() / 6
+
+
 def test_run_together_captured_and_on_another_stream(ops, gg):
     T, H, I, E, top_k = 70, 512, 256, 8, 2
     g = gen(70)

@@ -311,8 +311,10 @@ def quant_fp4(x: torch.Tensor, fmt: str = "nvfp4", global_scale: torch.Tensor | 
     """Quantises to 4-bit blocks: -> (codes uint8 [.., rows, K/2], scale tiles uint8 [.., *fp4_scale_shape(rows, K, fmt)]).
 
     x bf16/f16/f32 [rows, K] (row stride a multiple of 8) or, for operands of several groups, contiguous [G, rows, K].
-      fmt          "nvfp4": one e4m3 scale per 16 values under ``global_scale`` (f32, one value or [G]; default 1):
-                   s = e4m3(min(amax / (6 g), 448)), value = code * s * g.  "mxfp4": a power of two per 32 values
+      fmt          "nvfp4": one e4m3 scale per 16 values under ``global_scale`` (f32, one value or [G], positive and finite;
+                   default 1): s = e4m3(min(amax / (6 g), 448)), value = code * s * g.  "mxfp4": a power of two per 32 values
+      global_scale largest magnitude / (6 * 448) uses the scales' whole range.  With 1 a block whose largest magnitude is at
+                   most 0.0059 (6 * 2^-10) becomes zero: too large a factor for most weights
       act          "silu_mul": x is [rows, 2K] and SiLU(gate) * up, in fp32, is quantised (gate = the first half, or the
                    second with gate_first=False)
       src_pair     int32 [rows]: row r is made from x[src_pair[r] // top_k], as :func:`permute` gathers; where it is negative
