@@ -174,6 +174,30 @@ def test_norm_rows_whose_squares_pass_the_range(ops, dtype, H, residual):
     assert (scales[rest] == np.float32(1e-8) / np.float32(448)).all() and (codes[rest.repeat_interleave(128)[:H]] == 0).all()
 
 
+@pytest.mark.parametrize("pow2", [False, True])
+@pytest.mark.parametrize("mn", [False, True])
+@pytest.mark.parametrize("T,H,N", [(1, 256, 128), (300, 1024, 384)])
+def test_norm_feeds_the_grouped_product(ops, gg, T, H, N, pow2, mn):
+    """q and scales are the left operand of the 8-bit grouped product, in each of their layouts."""
+    from tirx_harness_b200.workloads import make_operand_b
+    x, r, w = _norm_inputs(T, H, "bf16", True, 0, 8)
+    n = ops.rms_norm_quant(x.cuda(), w.cuda(), residual=r.cuda(), pow2=pow2, mn_major=mn, want_y=True)
+    b, sb = make_operand_b(2, N, H, gen(9))
+    layout = (torch.arange(T, dtype=torch.int32) * 2) // T
+    d = torch.zeros((T, N), device="cuda")
+    gg.bind_contiguous(n["q"], n["scales"], b.cuda(), sb.cuda(), d, layout.cuda())()
+    assert gg.device_status() == 0
+    a = n["q"].float().cpu().double() * n["scales"].cpu().double().repeat_interleave(128, 1)
+    wide = b.float().double() * sb.double().repeat_interleave(128, 1)[:, :N].repeat_interleave(128, 2)
+    ref = torch.stack([a[t] @ wide[layout[t]].T for t in range(T)])
+    # that product's own tolerance: 1e-3 of the value, or of 2^-7 of the outputs' root mean square
+    within(d, ref, 1e-3 * torch.maximum(ref.abs(), 2.0**-7 * ref.square().mean().sqrt()), "product")
+    # and the operand stands for y: half a step of e4m3, or of its subnormals, and y's own rounding
+    y = n["y"].cpu().double()
+    s = n["scales"].cpu().double().repeat_interleave(128, 1)
+    assert ((a - y).abs() <= torch.maximum(2.0**-4 * y.abs(), 2.0**-10 * s) * (1 + 2.0**-6) + 2.0**-8 * y.abs()).all()
+
+
 @pytest.mark.parametrize("T,H,dtype,w32,dh", [(1, 7168, "bf16", False, True), (3, 8, "fp32", True, False), (517, 1000, "fp16", True, True),
                                               (700, 2048, "fp32", False, False), (300, 7168, "bf16", True, True), (5, 12296, "fp32", False, True),
                                               (6, 16384, "bf16", False, False)])
@@ -923,6 +947,35 @@ def _layer(ops, gg, x, res, wn, wr, bias, w13, w2, top_k, work):
     a2 = ops.quant_fp4(work["g1"], act="silu_mul")
     gg.bind_contiguous_fp4(*a2, *w2, work["y"], plan["grouped_layout"])()
     return dict(n=n, ids=ids, w=w, plan=plan, a1=a1, a2=a2, out=ops.combine(work["y"], plan["pos"], w))
+
+
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+@pytest.mark.parametrize("local", [256, 32, 4])
+def test_quant_fp4_of_a_plan_with_few_local_experts(ops, fmt, local):
+    """Gathered by a plan whose rows are mostly padding, as where few of the experts are on this GPU: x quantised once and copied,
+    or row by row, gives the same, and rows without a pair are zero."""
+    from tirx_harness_b200 import _lib
+    T, K, E, top_k = 1500, 1024, 256, 8
+    ids = torch.stack([torch.randperm(E, generator=gen(60 + t))[:top_k] for t in range(T)]).int()
+    plan = ops.permute_plan(ids.cuda(), 0, local)
+    x = torch.zeros((T, K)).normal_(generator=gen(27)).bfloat16()
+    rows = plan["cap_rows"]
+    assert _lib.lib().moe_quant_fp4_workspace_bytes(rows, T, K, 0) > 0
+    src = plan["src_pair"].cpu()
+    assert int((src >= 0).sum()) == int((ids < local).sum())
+    f = torch.tensor([1e-3], device="cuda") if fmt == "nvfp4" else None
+    q, sf = ops.quant_fp4(x.cuda(), fmt=fmt, global_scale=f, src_pair=plan["src_pair"], top_k=top_k)
+    rc, rb = quant32(x.float().numpy(), fmt, np.float32(1e-3) if fmt == "nvfp4" else 1.0)
+    live, t = (src >= 0).numpy(), (src // top_k).clamp(min=0).long().numpy()
+    b = scale_bytes(sf, rows, K, fmt)
+    np.testing.assert_array_equal(b[live], rb[t][live])
+    assert same_codes(codes_of(q)[live], rc[t][live])
+    assert not b[~live].any() and not q.cpu().numpy()[~live].any()
+    by_row, xd = (torch.zeros_like(q), torch.zeros_like(sf)), x.cuda()
+    _lib.FP4_QUANT(_lib.FP4_QUANT.pack(xd.data_ptr(), K, 0 if f is None else f.data_ptr(), 0, plan["src_pair"].data_ptr(), by_row[0].data_ptr(),
+                                       by_row[1].data_ptr(), 1, rows, T, K, top_k, 0, 0 if fmt == "nvfp4" else 1, 0, 1, 0, 0),
+                   torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(by_row[0], q) and torch.equal(by_row[1], sf)
 
 
 def test_product_of_quantised_weights_is_near_the_product_of_the_weights(ops, gg):
