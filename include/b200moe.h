@@ -288,11 +288,13 @@ int moe_rms_norm_backward(const moe_norm_grad_args* args, void* stream);
  * can be chosen; a group counts for its best p + bias or, with MOE_GROUP_TOP2, the sum of its two best.
  * weights = p * scale, or with renormalize p / (sum of the chosen p + 1e-20) * scale.
  * logits [T, E] of `dtype` (bf16, f16, f32), row stride in elements; bias [E] bf16 or f32; ids int32 and weights f32
- * [T, top_k], in descending order of p + bias.  The order is the exact one of p + bias, ties to the lowest index.
+ * [T, top_k], in descending order of p + bias.  The order is that of p + bias in 64 bits, without a bias that of the logits
+ * (which is p's, also where p rounds to 0 or 1); groups are compared in 64 bits; ties go to the lowest index, and -0 equals +0.
  * A logit or bias of -infinity or NaN switches its expert off, +infinity counts as the largest finite number; where fewer
  * than top_k experts are left the id is -1 and the weight 0, and moe_permute_plan drops the pair.  E <= 1024,
  * top_k <= min(32, E), n_group <= 32, and the kept groups hold at least top_k experts.
- * The general form of moe_route_topk and moe_route_deepseek (fp32 logits; their fixed rules). */
+ * The general form of moe_route_topk and moe_route_deepseek (fp32 logits; their fixed rules), which it outruns at every size;
+ * the layers below use those two. */
 #define MOE_SCORE_SOFTMAX 0
 #define MOE_SCORE_SIGMOID 1
 #define MOE_GROUP_MAX 0

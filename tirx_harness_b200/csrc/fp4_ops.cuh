@@ -78,8 +78,10 @@ template <> __device__ __forceinline__ float largest16<float>(const Raw8<float>&
     return __uint_as_float(m);
 }
 
-// x / (1 + exp(-x)) with the hardware's exp2 and reciprocal: off by less than 2^-20 of the value for |x| <= 20 (exp2 and
-// the rounding of its argument 2^-22 + |x| 2^-24 of 1 + exp, the reciprocal 2^-23), a thousandth of a 4-bit step.
+// x / (1 + exp(-x)) with the hardware's exp2 and reciprocal: off by at most (1.25 |x| + 8) 2^-24 of the value (exp2's argument
+// by the product's rounding and the constant's, 1.25 |x| 2^-24 of exp; exp2 4, the sum 1, the reciprocal 2, the product 1 times
+// 2^-24): 2e-6 at |x| = 20, a ten-thousandth of a 4-bit step.  From x = -87.4 down, where the value is below 2^-119, the
+// reciprocal is flushed and the result 0.
 __device__ __forceinline__ float silu_quick(float x) {
     float e, r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * -1.4426950408889634f));
@@ -253,6 +255,9 @@ __global__ void __launch_bounds__(FP4_QUANT_THREADS, sizeof(T) == 2 ? (SILU ? 3 
 // Where every row of x goes to several rows, its quantisation (53 us for 16384 x 7168 nvfp4, bound by instructions) and this
 // copy (bound by the L2 cache: it reads and writes 132 MB each in 36 us for 32768 rows) beat a quantisation of each row:
 // 16384 x 7168 in 2 rows each 113 -> 89 us, 4096 x 7168 in 8 rows each 108 -> 46 us.  FP4_COPY_FROM says from where on.
+// The rule counts rows, of which many may be padding: a plan of 16384 tokens with 8 of 256 experts each has 131072 rows and more
+// however few experts are local.  Copying is the faster way there too, because the other kernel pays for every block of rows, live
+// or not: 256, 32 and 4 local experts 188, 97 and 85 us against 475, 190 and 151.
 // Block: 64 rows x 1024 columns; a warp copies the 512 bytes of a row's codes and has eight rows under way.
 struct Fp4CopyParams {
     const uint8_t* q0; const uint32_t* sf0;     // sf0: row after row

@@ -8,7 +8,8 @@
 // CTAs' TMEM needs.  The scales come as the caller stores them, one contiguous piece per 128 rows and stage, and every
 // stage has TMEM columns of its own for them, so that the barrier that hands the stage over also covers them.  One
 // accumulator: two of 192 columns overlap the drain with the next tile's products but move 17 % more bytes per flop;
-// 28672 x 4096 x 7168 in 32 groups took 524 us with them and 507 us with this.
+// 28672 x 4096 x 7168 in 32 groups took 524 us with them and 507 us with this, both before the row blocks were paired (see
+// build_pair_list), under the power cap.  Two of 224 columns were not tried.
 #pragma once
 
 #include "fp4_ops.cuh"

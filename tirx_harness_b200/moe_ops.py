@@ -197,7 +197,9 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor
     dict(q e4m3 [T, H], scales f32 [T, ceil(H/128)], h, y, rstd f32 [T]) with h = round(x + residual) (x itself without a
     residual), y = h * rstd * weight (x's type; None unless ``want_y``) and q, scales its 1x128 quantisation as
     :func:`quant_1x128` does it, from y in fp32.  ``pow2`` rounds the scales up to powers of two, which the grouped GEMM
-    applies inside the tensor core; ``mn_major`` stores them [H/128, T].  H % 8 == 0, H <= 16384."""
+    applies inside the tensor core; ``mn_major`` stores them [H/128, T].  H % 8 == 0, H <= 16384.
+
+    Autograd does not see the call: the results carry no gradient, :func:`rms_norm_backward` computes it."""
     _check_float(x, "x")
     T, H, ld = _rows(x, "x")
     dt, dev = x.dtype, x.device
@@ -263,12 +265,16 @@ def route(logits: torch.Tensor, top_k: int, score: str = "softmax", bias: torch.
           topk_group: int = 1, group_score: str = "top2", renormalize: bool = True, scale: float = 1.0):
     """Top-k routing: bf16/f16/f32 [T, E] -> (ids int32 [T, top_k], weights f32 [T, top_k]).
 
-    p = softmax or sigmoid of the logits; the experts are chosen by p + bias (bf16/f32 [E]) in its exact order, ties to the
-    lowest index, and weighted by p (over its sum of the chosen with ``renormalize``) * scale.  With n_group > 1 only the
+    p = softmax or sigmoid of the logits; the experts are chosen by p + bias (bf16/f32 [E]) as 64 bits order it (without a
+    bias: in the logits' order), ties to the lowest index, and weighted by p (over its sum of the chosen with
+    ``renormalize``) * scale.  With n_group > 1 only the
     topk_group best groups of E / n_group consecutive experts count; a group's score is its best p + bias ("max") or the
     sum of its two best ("top2").  A logit or bias of -inf or NaN switches its expert off (+inf counts as the largest
     number); where fewer than top_k experts are left the id is -1 and the weight 0, which :func:`permute_plan` drops.
-    E <= 1024, top_k <= 32, n_group <= 32."""
+    E <= 1024, top_k <= 32, n_group <= 32.
+
+    It covers the rules of :func:`route_topk` and :func:`route_deepseek` and is faster than either at every size.  Autograd
+    does not see the call: the weights carry no gradient, :func:`route_backward` computes it."""
     _check_float(logits, "logits")
     T, E, ld = _rows(logits, "logits", 1)
     if bias is not None:
@@ -318,7 +324,8 @@ def quant_fp4(x: torch.Tensor, fmt: str = "nvfp4", global_scale: torch.Tensor | 
       act          "silu_mul": x is [rows, 2K] and SiLU(gate) * up, in fp32, is quantised (gate = the first half, or the
                    second with gate_first=False)
       src_pair     int32 [rows]: row r is made from x[src_pair[r] // top_k], as :func:`permute` gathers; where it is negative
-                   the row of ``out`` is left as it is
+                   the row of ``out`` is left as it is.  From twice as many rows as x has on, all of x is quantised once and
+                   its rows are copied, whatever share of the rows is negative
       out          (codes, scales) to write into; without it codes and scales of skipped rows are zero
     K % 128 == 0.  A block that holds an infinity or a NaN gets the scale NaN."""
     _check_float(x, "x")
